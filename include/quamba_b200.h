@@ -797,6 +797,153 @@ int qb_peer_put(const qb_peer_put_args* a, void* stream);
 int qb_peer_wait(const uint32_t* flags, int32_t n, uint32_t value, int32_t timeout_ms, void* stream);
 int qb_sum_partials(const void* partials, int32_t n_partials, int64_t partial_stride, void* out, int64_t n, void* stream);
 
+/* ---- selective scan in floating point, with gradients -----------------------------------------------------------------
+ * The Mamba1 recurrence of a float model (calibration, fine-tuning before quantisation), channel-last:
+ *   delta = dt_softplus ? softplus(dt + dt_bias) : dt + dt_bias
+ *   h_t   = exp(delta_t A) h_{t-1} + delta_t x_t B_t            (dim x dstate, float32)
+ *   y_t   = (sum_n C_t h_t + D x_t) silu(z_t)
+ * x, dt, z: (batch, seqlen, dim); Bm, Cm: (batch, seqlen, groups, dstate), channel d reads group d / (dim / groups); all of
+ * one type (dtype 0 float32, 1 float16, 2 bfloat16), unit stride in the last dim.  A (dim, dstate), D, dt_bias (dim),
+ * initial_state, final_state (batch, dim, dstate): float32, contiguous; D, dt_bias, z, initial_state, final_state may be
+ * NULL.  lengths (batch) int32 on the device, or NULL: tokens from lengths[b] on are not part of sequence b -- what lies
+ * there is not used, y and every gradient is 0 there; values outside 0..seqlen count as the nearer end.  1 <= dstate <= 64.
+ * y and the gradients of x, dt, z, B, C are contiguous.
+ *
+ * qb_float_scan_fwd: y and final_state; with checkpoints != NULL also the states every 16 tokens, in the library's own
+ *   order (qb_float_scan_checkpoint_bytes), for the backward pass.
+ * qb_float_scan_bwd: reads the forward pass's inputs and checkpoints, dy (y's type and shape) and d_final (NULL: zero);
+ *   writes d_x, d_dt, d_B, d_C, d_z (with z), d_A, d_D, d_bias (each may be NULL) and d_initial (may be NULL).  Sums over channels,
+ *   tokens and sequences are taken in float32 in a fixed order: the same call gives the same bits.
+ * Both take a workspace of qb_float_scan_workspace_bytes(..., backward); one workspace serves one call at a time. */
+typedef struct {
+  const void* x;
+  const void* dt;
+  const void* z;
+  const void* Bm;
+  const void* Cm;
+  const float* A;
+  const float* D;
+  const float* dt_bias;
+  const float* initial_state;
+  const int32_t* lengths;
+  void* y;
+  float* final_state;
+  float* checkpoints;
+  const void* dy;
+  const float* d_final;
+  void* d_x;
+  void* d_dt;
+  void* d_z;
+  void* d_B;
+  void* d_C;
+  float* d_A;
+  float* d_D;
+  float* d_bias;
+  float* d_initial;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t x_sb;
+  int64_t x_sl;
+  int64_t dt_sb;
+  int64_t dt_sl;
+  int64_t z_sb;
+  int64_t z_sl;
+  int64_t B_sb;
+  int64_t B_sl;
+  int64_t B_sg;
+  int64_t C_sb;
+  int64_t C_sl;
+  int64_t C_sg;
+  int64_t dy_sb;
+  int64_t dy_sl;
+  int32_t batch;
+  int32_t seqlen;
+  int32_t dim;
+  int32_t dstate;
+  int32_t groups;
+  int32_t dtype;
+  int32_t dt_softplus;
+} qb_float_scan_args;
+int64_t qb_float_scan_checkpoint_bytes(int32_t batch, int32_t seqlen, int32_t dim, int32_t groups, int32_t dstate);
+int64_t qb_float_scan_workspace_bytes(int32_t batch, int32_t seqlen, int32_t dim, int32_t groups, int32_t dstate, int32_t backward);
+int qb_float_scan_fwd(const qb_float_scan_args* a, void* stream);
+int qb_float_scan_bwd(const qb_float_scan_args* a, void* stream);
+
+/* The same recurrence by one token per sequence: x, dt, z, y (batch, dim), Bm, Cm (batch, groups, dstate), state float32
+ * (batch, dim, dstate) with unit stride in the last dim.  The new state goes to state_out, which may be state itself. */
+typedef struct {
+  const float* state;
+  float* state_out;
+  const void* x;
+  const void* dt;
+  const void* z;
+  const void* Bm;
+  const void* Cm;
+  const float* A;
+  const float* D;
+  const float* dt_bias;
+  void* y;
+  int64_t state_sb;
+  int64_t state_sd;
+  int64_t state_out_sb;
+  int64_t state_out_sd;
+  int64_t x_sb;
+  int64_t dt_sb;
+  int64_t z_sb;
+  int64_t B_sb;
+  int64_t B_sg;
+  int64_t C_sb;
+  int64_t C_sg;
+  int32_t batch;
+  int32_t dim;
+  int32_t dstate;
+  int32_t groups;
+  int32_t dtype;
+  int32_t dt_softplus;
+} qb_float_update_args;
+int qb_float_scan_update(const qb_float_update_args* a, void* stream);
+
+/* ---- log probabilities of given tokens ----------------------------------------------------------------------------------
+ * For each row of logits (dtype 0 float32, 1 float16, 2 bfloat16; unit stride inside a row; row r begins at element
+ * (r / inner_rows) * outer_stride + (r % inner_rows) * row_stride, so that a slice of (batch, seqlen, vocab) needs no copy):
+ *   lse        = log sum_i exp(x_i)                              logprobs[r] = x_target - lse
+ *   entropy[r] = lse - sum_i p_i x_i, p_i = exp(x_i - lse)       (entropy may be NULL)
+ *   top_logprobs / top_ids (rows, top_k): the top_k largest logits' log probabilities and columns, largest first, equal
+ *   values in the order of their columns; 0 <= top_k <= 32, top_k <= vocab.
+ * A column of -inf has probability 0.  A row of nothing but -inf has no distribution: log probabilities -inf, entropy 0 and
+ * gradient 0.  A row that holds a NaN or +inf gives NaN (and some columns of the row as top_ids).  targets int64 (rows): ignore_index
+ * gives logprobs 0 without gradient; any other value outside 0..vocab-1 gives NaN and sets the device status word.
+ * lse (rows) float32 keeps what the backward pass needs (may be NULL in the forward pass).
+ * qb_logprobs_bwd: d_logits = g ([i == target] - p_i) - h p_i (log p_i + H) for the gradients g (d_logprobs) and h
+ *   (d_entropy) of a row's two results, either of which may be NULL; reads entropy where d_entropy is given; d_logits in the
+ *   logits' type, its rows placed by d_outer_stride and d_row_stride (fastest where they start at the same offset from a
+ *   16-byte boundary as the logits' rows). */
+typedef struct {
+  const void* logits;
+  const int64_t* targets;
+  float* logprobs;
+  float* entropy;
+  float* lse;
+  float* top_logprobs;
+  int64_t* top_ids;
+  const float* d_logprobs;
+  const float* d_entropy;
+  void* d_logits;
+  int64_t outer_stride;
+  int64_t row_stride;
+  int64_t d_outer_stride;
+  int64_t d_row_stride;
+  int64_t ignore_index;
+  int64_t rows;
+  int64_t inner_rows;
+  int32_t vocab;
+  int32_t top_k;
+  int32_t dtype;
+} qb_logprobs_args;
+#define QB_LOGPROBS_MAX_TOP 32
+int qb_logprobs_fwd(const qb_logprobs_args* a, void* stream);
+int qb_logprobs_bwd(const qb_logprobs_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@ reference's own extension-level and module-level interfaces:
         W4A8B16O16Linear, W4A8B8O8Linear, W4A8B8O8LinearParallel, W8A8B8O8Linear, \
         W8A8B8O8LinearParallel, W8A8B16O16Linear, QRMSNorm, QRMSNormGated, W4O16Embedding, W8O16Embedding, \
         W4A8QMamba2, W8A8QMamba2, W4A8QMamba, W8A8QMamba, QuambaLMHeadModel
+    from quamba_b200 import selective_scan, selective_scan_update, token_logprobs      # float models, scores and losses
 
 Importing the package does not touch the GPU; the shared library is loaded on first use and
 its absence is an error (there is no CPU or PyTorch fallback).
@@ -19,6 +20,8 @@ from .modules import (QCausalConv1D, QHadamard, QSScan, Quamb2Conv1D, Quamba2Chu
                       W8A8B8O8LinearParallel, W8A8B16O16Linear)
 from .packing import w4a8_quantize  # noqa: F401
 from .norm import QRMSNorm, QRMSNormGated  # noqa: F401
+from .scan import selective_scan, selective_scan_update  # noqa: F401
+from .scoring import TokenLogprobs, token_logprobs  # noqa: F401
 from .embedding import W4O16Embedding, W8O16Embedding  # noqa: F401
 from .mixer import W4A8QMamba2, W8A8QMamba2  # noqa: F401
 from .mixer1 import QAct, W4A8QMamba, W8A8QMamba  # noqa: F401

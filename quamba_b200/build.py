@@ -19,8 +19,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libquamba_b200.so"
 NATIVE = PKG / ("_native" + sysconfig.get_config_var("EXT_SUFFIX"))
 SOURCES = ["lib.cu", "conv1d.cu", "hadamard.cu", "hadamard_tc.cu", "sscan.cu", "sscan_cl.cu", "ssd.cu", "ssd_tc.cu", "linear.cu", "gemm_tc.cu", "norm.cu",
-           "embedding.cu", "decode.cu", "peer.cu"]
-NATIVE_SOURCES = ["binding.cpp", "binding_layers.cpp"]
+           "embedding.cu", "decode.cu", "peer.cu", "fscan.cu", "logprobs.cu"]
+NATIVE_SOURCES = ["binding.cpp", "binding_layers.cpp", "binding_float.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas", "-v"]
 CUDA = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))

@@ -239,5 +239,10 @@ void w4a8_run(PyObject* prep, const W4Dims& w, const int8_t* a, int64_t lda, int
 
 PyObject* mamba2_layer(const Args& a);
 PyObject* mamba1_layer(const Args& a);
+PyObject* float_scan_fwd(const Args& a);
+PyObject* float_scan_bwd(const Args& a);
+PyObject* float_scan_update(const Args& a);
+PyObject* logprobs_fwd(const Args& a);
+PyObject* logprobs_bwd(const Args& a);
 
 }  // namespace qbn

@@ -67,6 +67,10 @@ extern "C" int qb_read_device_status(void* stream) {
       qb::set_error("embedding_lookup met a token id outside the table (code %d)", v);
       return QB_ERR_INVALID_ARG;
     }
+    if (v == 502) {
+      qb::set_error("token_logprobs met a target outside the vocabulary (code %d)", v);
+      return QB_ERR_INVALID_ARG;
+    }
     qb::set_error("a bounded device-side wait expired (code %d)", v);
     return QB_ERR_TIMEOUT;
   }
@@ -109,6 +113,9 @@ extern "C" int64_t qb_sizeof(const char* name) {
   QB_SZ(qb_decode_norm_linear_args);
   QB_SZ(qb_decode_gate_had_quant_args);
   QB_SZ(qb_peer_put_args);
+  QB_SZ(qb_float_scan_args);
+  QB_SZ(qb_float_update_args);
+  QB_SZ(qb_logprobs_args);
 #undef QB_SZ
   return -1;
 }
