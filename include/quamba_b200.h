@@ -809,7 +809,7 @@ int qb_sum_partials(const void* partials, int32_t n_partials, int64_t partial_st
  * there is not used, y and every gradient is 0 there; values outside 0..seqlen count as the nearer end.  1 <= dstate <= 64.
  * y and the gradients of x, dt, z, B, C are contiguous.
  *
- * qb_float_scan_fwd: y and final_state; with checkpoints != NULL also the states every 16 tokens, in the library's own
+ * qb_float_scan_fwd: y and final_state; with checkpoints != NULL also the states every 8 tokens, in the library's own
  *   order (qb_float_scan_checkpoint_bytes), for the backward pass.
  * qb_float_scan_bwd: reads the forward pass's inputs and checkpoints, dy (y's type and shape) and d_final (NULL: zero);
  *   writes d_x, d_dt, d_B, d_C, d_z (with z), d_A, d_D, d_bias (each may be NULL) and d_initial (may be NULL).  Sums over channels,

@@ -2,33 +2,34 @@
 //
 //   delta = softplus(dt + bias), h_t[n] = exp(delta_t A[n]) h_{t-1}[n] + delta_t x_t B_t[n], y_t = (C_t . h_t + D x_t) silu(z_t)
 //
-// A warp owns 512 states of one sequence: 8 groups of lanes x 4 lanes; the four lanes of a group share kCh channels and hold
-// kNp consecutive states of each (kCh * kNp = 16 states a lane).  So the states' sums over n are shuffles between four lanes,
-// what a token's B and C cost is one 128-bit read each for all channels of a lane, and in the backward pass the sums over
-// channels (dB, dC) are taken in the lane first and then between eight lanes.  States and sums are float32 throughout, walked in
-// packed pairs.
+// A warp owns a tile of channels of one sequence (or of a segment of it).  kQ lanes share kCh channels and hold kNp consecutive
+// states of each: the states' sums over n are shuffles between two or four lanes, what a token's B and C cost is one or two
+// 128-bit reads for all channels of a lane, and in the backward pass the sums over channels (dB, dC) are taken in the lane, then
+// between the lanes, then over the CTA.  States and sums are float32 throughout, walked in packed pairs.
 //
 // Bound: dstate exponentials per (token, channel) on the MUFU pipe (16 results per clock and SM): 16 states cost 1 clock per
 // (token, channel) and SM, while its bytes (8 at 16 bits) take 0.18 clocks of HBM time.
 #include <algorithm>
-#include "common.cuh"
+#include "tc_common.cuh"
 
 namespace qb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kCkpt = 16;              // tokens between two kept states
-constexpr int kRec = 512;              // states of a warp
-constexpr int kSum = kRec + 32;        // a segment's summary: its states from zero, and the summed delta of its channels
-constexpr int kGrad = kRec + 64;       // a warp's sums for dA | dD | d_bias
+constexpr float kLift = 3.0e-8f;       // of the exponential unit: see make_up()
+constexpr int kCkpt = 8;               // tokens between two kept states
 constexpr int kBwdWarps = 4;
 
-template <typename T, int kNp_>
+// kQ lanes share kCh channels; each holds kNp consecutive states of them.
+template <int kNp_, int kCh_, int kQ_>
 struct Geo {
-  static constexpr int kNp = kNp_, kPairs = kNp / 2, kCh = 16 / kNp, kWc = 8 * kCh, kN = 4 * kNp;
+  static constexpr int kNp = kNp_, kPairs = kNp / 2, kCh = kCh_, kQ = kQ_, kWc = 32 / kQ * kCh, kN = kQ * kNp;
   static constexpr int kLanesRow = kWc / 4;             // lanes that hold one token's channels, four each
   static constexpr int kRows = 32 / kLanesRow;          // tokens per warp-wide access
+  static constexpr int kRec = 32 * kNp * kCh;           // states of a warp
+  static constexpr int kSum = kRec + 32;                // a segment's summary: its states from zero, and the summed delta of its channels
+  static constexpr int kGrad = kRec + 64;               // a warp's sums for dA | dD | d_bias
 };
 
 __device__ __forceinline__ float rcp_fast(float x) {
@@ -36,19 +37,22 @@ __device__ __forceinline__ float rcp_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// max(v, 0) + log1p(e), e = exp(-|v|); log1p(e) = 2 artanh(s) with s = e / (2 + e) <= 1/3, by its series up to s^15 (the next
-// term is below 2^-29 of the sum).
-__device__ __forceinline__ float softplus_series(float v) {
-  const float e = fast_exp2(-fabsf(v) * kLog2e);
-  const float s = e * rcp_fast(2.0f + e), w = s * s;
-  float p = fmaf(w, 1.0f / 15, 1.0f / 13);
-  p = fmaf(w, p, 1.0f / 11);
-  p = fmaf(w, p, 1.0f / 9);
-  p = fmaf(w, p, 1.0f / 7);
-  p = fmaf(w, p, 1.0f / 5);
-  p = fmaf(w, p, 1.0f / 3);
-  p = fmaf(w, p, 1.0f);
-  return fmaf(2.0f * s, p, fmaxf(v, 0.0f));
+__device__ __forceinline__ f2 splat(float v) { return pack2(v, v); }
+// max(v, 0) + log1p(e), e = exp(-|v|), for two values; log1p(e) = 2 artanh(s) with s = e / (2 + e) <= 1/3, by its series up to s^15
+// (the next term is below 2^-29 of the sum).
+__device__ __forceinline__ void softplus_series(float& a, float& b) {
+  const f2 e = pack2(fast_exp2(-fabsf(a) * kLog2e), fast_exp2(-fabsf(b) * kLog2e));
+  float x, y;
+  unpack2(add2(e, splat(2.0f)), x, y);
+  const f2 s = mul2(e, pack2(rcp_fast(x), rcp_fast(y))), w = mul2(s, s);
+  f2 p = fma2(w, splat(1.0f / 15), splat(1.0f / 13));
+  p = fma2(w, p, splat(1.0f / 11));
+  p = fma2(w, p, splat(1.0f / 9));
+  p = fma2(w, p, splat(1.0f / 7));
+  p = fma2(w, p, splat(1.0f / 5));
+  p = fma2(w, p, splat(1.0f / 3));
+  p = fma2(w, p, splat(1.0f));
+  unpack2(fma2(add2(s, s), p, pack2(fmaxf(a, 0.0f), fmaxf(b, 0.0f))), a, b);
 }
 __device__ __forceinline__ float sigmoid_fast(float v) {
   const float e = fast_exp2(-fabsf(v) * kLog2e), r = rcp_fast(1.0f + e);
@@ -58,6 +62,22 @@ __device__ __forceinline__ f2 exp2_pair(f2 x) {
   float a, b;
   unpack2(x, a, b);
   return pack2(fast_exp2(a), fast_exp2(b));
+}
+
+// 2^x to within rounding: the nearest integer by the adder, the fraction's power by its series (|f| <= 1/2, the term left out is
+// below 2^-27).  Results below 2^-126 are zero, above 2^127 infinite.
+__device__ __forceinline__ float exp2_series(float x) {
+  const float c = fminf(fmaxf(x, -127.0f), 128.0f);
+  const float i = rintf(c), f = (c - i) * kLn2;
+  float p = fmaf(f, 1.0f / 5040, 1.0f / 720);
+  p = fmaf(f, p, 1.0f / 120);
+  p = fmaf(f, p, 1.0f / 24);
+  p = fmaf(f, p, 1.0f / 6);
+  p = fmaf(f, p, 0.5f);
+  p = fmaf(f, p, 1.0f);
+  p = fmaf(f, p, 1.0f);
+  const float r = p * __int_as_float(((int)i + 127) << 23);       // exponent 0: zero, 255: infinite
+  return x != x ? x : r;
 }
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -74,7 +94,7 @@ __device__ __forceinline__ float4 quad(const T* p) {
   if constexpr (sizeof(T) == 4) {
     return *reinterpret_cast<const float4*>(p);
   } else {
-    T v[4];
+    __align__(8) T v[4];
     *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p);
     return make_float4(to_f(v[0]), to_f(v[1]), to_f(v[2]), to_f(v[3]));
   }
@@ -88,15 +108,32 @@ template <int kPending>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
 
 // `count` of four consecutive values to shared memory
-template <typename T>
-__device__ __forceinline__ void stage_quad(T* dst, const T* src, int count, bool vec) {
-  if (count <= 0) return;
-  if (vec) {
-    copy_async<4 * sizeof(T)>(dst, src);
+template <bool kVec, typename T>
+__device__ __forceinline__ void stage_quad(T* dst, const T* src, int count) {
+  if constexpr (kVec) {
+    if (count > 0) copy_async<4 * sizeof(T)>(dst, src);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (k < count) dst[k] = src[k];
+  }
+}
+
+// four consecutive values to global memory, `count` of them where they do not lie together
+template <typename T>
+__device__ __forceinline__ void store_quad(T* dst, const float (&v)[4], int count, bool vec) {
+  __align__(16) T r[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) r[k] = from_f<T>(v[k]);
+  if (vec) {
+    if (count > 0) {
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(r);
+      else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(r);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < count) dst[k] = r[k];
   }
 }
 
@@ -123,21 +160,65 @@ __device__ __forceinline__ void load_channels(const float* p, float (&v)[kCh]) {
   }
 }
 
-// v[c] summed over the four lanes of a group; the lane gets the total of its own channel, q * kCh / 4
-template <int kCh>
+// v[c] summed over the kQ lanes of a group; the lane gets the total of the channel Place::own
+template <int kCh, int kQ>
 __device__ __forceinline__ float own_channel(const float (&v)[kCh], int q) {
-  const bool hi = q & 2, odd = q & 1;
-  if constexpr (kCh == 4) {
-    const float a = (hi ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 2);
-    const float b = (hi ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 2);
-    return (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
-  } else if constexpr (kCh == 2) {
-    const float a = (hi ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[1], 2);
-    return a + __shfl_xor_sync(0xffffffffu, a, 1);
-  } else {
-    const float a = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 2);
-    return a + __shfl_xor_sync(0xffffffffu, a, 1);
+  float a = v[0];
+  int bit = kQ / 2;
+  if constexpr (kCh == 2) {
+    const bool hi = q & bit;
+    a = (hi ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[1], bit);
+    bit /= 2;
   }
+#pragma unroll
+  for (; bit > 0; bit /= 2) a += __shfl_xor_sync(0xffffffffu, a, bit);
+  return a;
+}
+
+// v summed over the lanes of one q, which halve the list between them until it has one value; the sums go to out
+template <int kCount, int kQ>
+__device__ __forceinline__ void over_groups(float (&v)[kCount], int lane, float* out) {
+  int at = 0, left = kCount;
+#pragma unroll
+  for (int bit = 16; bit >= kQ; bit >>= 1) {
+    const bool up = lane & bit;
+    if (left > 1) {
+      left /= 2;
+#pragma unroll
+      for (int k = 0; k < left; ++k) v[k] = (up ? v[left + k] : v[k]) + __shfl_xor_sync(0xffffffffu, up ? v[k] : v[left + k], bit);
+      at += up ? left : 0;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);     // both hold the sum
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < left; ++k) out[at + k] = v[k];
+}
+
+// a token's decays, and its step of the states
+template <typename G>
+__device__ __forceinline__ void decays(const float (&d)[G::kCh], const f2 (&A)[G::kCh][G::kPairs], f2 (&e)[G::kCh][G::kPairs]) {
+  const f2 lift = pack2(kLift, kLift);                   // see make_up()
+#pragma unroll
+  for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+    for (int p = 0; p < G::kPairs; ++p) e[c][p] = fma2(pack2(d[c], d[c]), A[c][p], lift);
+#pragma unroll
+  for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+    for (int p = 0; p < G::kPairs; ++p) e[c][p] = exp2_pair(e[c][p]);
+}
+template <typename G>
+__device__ __forceinline__ void advance(const f2 (&e)[G::kCh][G::kPairs], const float (&u)[G::kCh], const f2 (&b2)[G::kPairs], f2 (&h)[G::kCh][G::kPairs]) {
+  f2 in[G::kCh][G::kPairs];
+#pragma unroll
+  for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+    for (int p = 0; p < G::kPairs; ++p) in[c][p] = mul2(b2[p], pack2(u[c], u[c]));
+#pragma unroll
+  for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+    for (int p = 0; p < G::kPairs; ++p) h[c][p] = fma2(e[c][p], h[c][p], in[c][p]);
 }
 
 // where a warp stands
@@ -146,17 +227,15 @@ struct Place {
   int lane, q, cg;
   int b, seg, ch0, nch, group, tile;                     // the tile's first channel and how many exist
   int own;                                               // the channel (of the tile) whose sums this lane gets
-  bool writes;
   __device__ __forceinline__ Place(const qb_float_scan_args& a, int tpg, int b_, int seg_, int tile_, int lane_) {
-    lane = lane_; q = lane & 3; cg = lane >> 2;
+    lane = lane_; q = lane % G::kQ; cg = lane / G::kQ;
     b = b_; seg = seg_; tile = tile_;
     const int per = a.dim / a.groups;
     group = tile / tpg;
     const int c0 = (tile % tpg) * G::kWc;
     ch0 = group * per + c0;
     nch = min(G::kWc, per - c0);
-    own = cg * G::kCh + q * G::kCh / 4;
-    writes = q % (4 / G::kCh) == 0 && own < nch;
+    own = cg * G::kCh + q * G::kCh / G::kQ;
   }
 };
 
@@ -202,22 +281,48 @@ __device__ __forceinline__ void store_state(float* s, const qb_float_scan_args& 
       if (n + 1 < a.dstate) row[1] = y;
     }
 }
-// the same in the library's own order, 16 bytes per lane and access
+// a warp's states one after another, 16 bytes per lane and access
 template <typename G, typename P>
 __device__ __forceinline__ void load_record(const P* rec, int lane, f2 (&h)[G::kCh][G::kPairs]) {
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
+  for (int i = 0; i < G::kCh * G::kPairs; i += 2) {
     const ulonglong2 v = *(reinterpret_cast<const ulonglong2*>(rec) + (i / 2) * 32 + lane);
     h[i / G::kPairs][i % G::kPairs] = v.x;
-    h[(i + 1) / G::kPairs][(i + 1) % G::kPairs] = v.y;
+    h[i / G::kPairs][i % G::kPairs + 1] = v.y;
   }
 }
 template <typename G, typename P>
 __device__ __forceinline__ void store_record(P* rec, int lane, const f2 (&h)[G::kCh][G::kPairs]) {
 #pragma unroll
-  for (int i = 0; i < 8; i += 2)
-    *(reinterpret_cast<ulonglong2*>(rec) + (i / 2) * 32 + lane) =
-        make_ulonglong2(h[i / G::kPairs][i % G::kPairs], h[(i + 1) / G::kPairs][(i + 1) % G::kPairs]);
+  for (int i = 0; i < G::kCh * G::kPairs; i += 2)
+    *(reinterpret_cast<ulonglong2*>(rec) + (i / 2) * 32 + lane) = make_ulonglong2(h[i / G::kPairs][i % G::kPairs], h[i / G::kPairs][i % G::kPairs + 1]);
+}
+// kept states lie as (batch, chunk, dim, 4 kNp), whatever a warp's share of the channels is
+template <typename G>
+__device__ __forceinline__ int64_t kept_at(const qb_float_scan_args& a, const Place<G>& w, int chunk) {
+  return (((int64_t)w.b * ((a.seqlen + kCkpt - 1) / kCkpt) + chunk) * a.dim + w.ch0 + w.cg * G::kCh) * G::kN + w.q * G::kNp;
+}
+template <typename G>
+__device__ __forceinline__ void load_kept(const qb_float_scan_args& a, const Place<G>& w, int chunk, f2 (&h)[G::kCh][G::kPairs]) {
+  const float* at = a.checkpoints + kept_at(a, w, chunk);
+#pragma unroll
+  for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+    for (int p = 0; p < G::kPairs; p += 2) {
+      ulonglong2 v = make_ulonglong2(0ull, 0ull);
+      if (w.cg * G::kCh + c < w.nch) v = *reinterpret_cast<const ulonglong2*>(at + c * G::kN + 2 * p);
+      h[c][p] = v.x;
+      h[c][p + 1] = v.y;
+    }
+}
+template <typename G>
+__device__ __forceinline__ void store_kept(const qb_float_scan_args& a, const Place<G>& w, int chunk, const f2 (&h)[G::kCh][G::kPairs]) {
+  float* at = a.checkpoints + kept_at(a, w, chunk);
+#pragma unroll
+  for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+    for (int p = 0; p < G::kPairs; p += 2)
+      if (w.cg * G::kCh + c < w.nch) *reinterpret_cast<ulonglong2*>(at + c * G::kN + 2 * p) = make_ulonglong2(h[c][p], h[c][p + 1]);
 }
 // h <- what the summarised segment makes of it
 template <typename G>
@@ -226,15 +331,53 @@ __device__ __forceinline__ void fold(const float* sum, const Place<G>& w, const 
   load_record<G>(sum, w.lane, loc);
 #pragma unroll
   for (int c = 0; c < G::kCh; ++c) {
-    const float d = sum[kRec + w.cg * G::kCh + c];
+    const float d = sum[G::kRec + w.cg * G::kCh + c];
 #pragma unroll
     for (int p = 0; p < G::kPairs; ++p) h[c][p] = fma2(exp2_pair(mul2(pack2(d, d), A[c][p])), h[c][p], loc[c][p]);
+  }
+}
+
+// The exponential unit's results are low by 2.1e-8 of their value on average, one sign for all, which a state that lives for
+// tens of tokens would lose for each of them; the exponent's fma adds that much (kLift).  For arguments in (-1/64, 0), where states
+// live for hundreds of tokens, the mean error varies with the argument, by +-1.5e-8, and down to -3/64 it is a little larger:
+// the difference is given back once for a tile of `tokens`, in its middle.  delta2 is the sum of two of the tile's deltas.  (The
+// line below follows the mean error of 2^18 random arguments in each of 20 intervals.  Without all this the gradient of A is
+// off by 2.8e-6, with it by less than 1e-6; a polynomial in place of the unit would cost 40% more instructions.)
+template <typename G>
+__device__ __forceinline__ void make_up(const float (&delta2)[G::kCh], float tokens, const f2 (&A)[G::kCh][G::kPairs], f2 (&h)[G::kCh][G::kPairs]) {
+  const f2 rise = splat(3.4e-6f * tokens), rise0 = splat(-2.2e-8f * tokens);
+  const float least = -1.51e-8f * tokens, most = 1.05e-8f * tokens, mid = 0.6e-8f * tokens;
+#pragma unroll
+  for (int c = 0; c < G::kCh; ++c) {
+    const f2 half = splat(-0.5f * delta2[c]);
+#pragma unroll
+    for (int p = 0; p < G::kPairs; ++p) {
+      const f2 arg = mul2(half, A[c][p]);                // A is negative
+      float x, y, ux, uy;
+      unpack2(arg, x, y);
+      unpack2(fma2(arg, rise, rise0), ux, uy);
+      ux = x < 1.0f / 64 ? fmaxf(fminf(ux, most), least) : x < 3.0f / 64 ? mid : 0.0f;
+      uy = y < 1.0f / 64 ? fmaxf(fminf(uy, most), least) : y < 3.0f / 64 ? mid : 0.0f;
+      h[c][p] = fma2(h[c][p], pack2(ux, uy), h[c][p]);
+    }
   }
 }
 
 __device__ __forceinline__ int live_tokens(const qb_float_scan_args& a, int b) {
   return a.lengths != nullptr ? max(0, min(a.seqlen, a.lengths[b])) : a.seqlen;
 }
+
+// four tokens' or channels' delta before what is not there is left out
+__device__ __forceinline__ void deltas(const float4& raw, const float (&bias)[4], int softplus, float (&d)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) d[k] = (k == 0 ? raw.x : k == 1 ? raw.y : k == 2 ? raw.z : raw.w) + bias[k];
+  if (softplus) {
+    softplus_series(d[0], d[1]);
+    softplus_series(d[2], d[3]);
+  }
+}
+
+struct Vec { int wide, bc; };           // whether four consecutive values can be moved together
 
 // Raw rows of a tile of tokens, as they lie in memory.
 template <typename T, typename G, int kT, int kWide>
@@ -243,25 +386,37 @@ struct Raw {
   T bc[2][kT][G::kN];
 };
 // stages tokens t0 .. min(t0 + kT, end) - 1
-template <typename T, typename G, int kT, int kWide>
-__device__ __forceinline__ void stage_tile(Raw<T, G, kT, kWide>& raw, const T* const (&src)[kWide], const int64_t (&stride)[kWide], const T* const (&bc)[2],
-                                           const int64_t (&bc_stride)[2], int t0, int end, int nch, int dstate, bool vec, bool vec_bc, int lane) {
+template <bool kVec, typename T, typename G, int kT, int kWide>
+__device__ __forceinline__ void stage_wide(Raw<T, G, kT, kWide>& raw, const T* const (&src)[kWide], const int64_t (&stride)[kWide], int t0, int end, int nch, int lane) {
   const int row = lane / G::kLanesRow, c4 = (lane % G::kLanesRow) * 4;
 #pragma unroll
-  for (int i = 0; i < kT / G::kRows; ++i) {
-    const int t = i * G::kRows + row;
-    if (t0 + t < end) {
+  for (int k = 0; k < kWide; ++k) {
+    if (src[k] == nullptr) continue;
+    const T* at = src[k] + (int64_t)(t0 + row) * stride[k] + c4;
 #pragma unroll
-      for (int k = 0; k < kWide; ++k)
-        if (src[k] != nullptr) stage_quad(&raw.wide[k][t][c4], src[k] + (int64_t)(t0 + t) * stride[k] + c4, nch - c4, vec);
+    for (int i = 0; i < (kT + G::kRows - 1) / G::kRows; ++i) {
+      const int t = i * G::kRows + row;
+      if (t < kT && t0 + t < end) stage_quad<kVec>(&raw.wide[k][t][c4], at + i * G::kRows * stride[k], nch - c4);
     }
   }
+}
+template <bool kVec, typename T, typename G, int kT, int kWide>
+__device__ __forceinline__ void stage_bc(Raw<T, G, kT, kWide>& raw, const T* const (&bc)[2], const int64_t (&stride)[2], int t0, int end, int dstate, int lane) {
   constexpr int kQuads = G::kN / 4;
 #pragma unroll
   for (int i = 0; i < 2 * kT * kQuads / 32; ++i) {
     const int e = i * 32 + lane, n4 = (e % kQuads) * 4, t = (e / kQuads) % kT, k = e / kQuads / kT;
-    if (t0 + t < end && bc[k] != nullptr) stage_quad(&raw.bc[k][t][n4], bc[k] + (int64_t)(t0 + t) * bc_stride[k] + n4, dstate - n4, vec_bc);
+    const T* from = k ? bc[1] : bc[0];
+    if (t0 + t < end && from != nullptr) stage_quad<kVec>(&raw.bc[k][t][n4], from + (int64_t)(t0 + t) * (k ? stride[1] : stride[0]) + n4, dstate - n4);
   }
+}
+template <typename T, typename G, int kT, int kWide>
+__device__ __forceinline__ void stage_tile(Raw<T, G, kT, kWide>& raw, const T* const (&src)[kWide], const int64_t (&stride)[kWide], const T* const (&bc)[2],
+                                           const int64_t (&bc_stride)[2], int t0, int end, int nch, int dstate, Vec vec, int lane) {
+  if (vec.wide) stage_wide<true, T, G, kT, kWide>(raw, src, stride, t0, end, nch, lane);
+  else stage_wide<false, T, G, kT, kWide>(raw, src, stride, t0, end, nch, lane);
+  if (vec.bc) stage_bc<true, T, G, kT, kWide>(raw, bc, bc_stride, t0, end, dstate, lane);
+  else stage_bc<false, T, G, kT, kWide>(raw, bc, bc_stride, t0, end, dstate, lane);
 }
 // widens a tile's B and C, zero outside the sequence and past dstate
 template <typename T, typename G, int kT, typename R>
@@ -281,7 +436,6 @@ __device__ __forceinline__ void widen_bc(const R& raw, float (&out)[2][kT][G::kN
 }
 __device__ __forceinline__ float at(const float4& v, int k) { return k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w; }
 
-struct Vec { int wide, bc; };
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 template <typename T, typename G>
@@ -294,12 +448,11 @@ struct FwdSmem {
 
 // One warp: a tile of channels of one segment of one sequence.  kMode 0: outputs (from the folded summaries of the segments
 // before); 1: the segment's summary; 2: the summary of the backward recurrence, from the segment's end to its start.
-template <typename T, int kNp, int kMode>
-__global__ void __launch_bounds__(32)
+template <typename T, typename G, int kMode>
+__global__ void __launch_bounds__(32, G::kRec == 512 ? 20 : 28)
 float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nseg, int seg_len, float* sums, Vec vec) {
-  using G = Geo<T, kNp>;
   using S = FwdSmem<T, G>;
-  constexpr int kT = S::kT;
+  constexpr int kT = S::kT, kNp = G::kNp;
   constexpr bool kOut = kMode == 0, kRev = kMode == 2;
   extern __shared__ __align__(16) unsigned char dyn[];
   S& s = *reinterpret_cast<S*>(dyn);
@@ -315,7 +468,8 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
   load_A(a, w, A);
   load_state(kOut ? a.initial_state : nullptr, a, w, h);
   if (kOut)
-    for (int i = 0; i < w.seg; ++i) fold(sums + (((int64_t)w.b * nseg + i) * tiles + w.tile) * kSum, w, A, h);
+#pragma unroll 4
+    for (int i = 0; i < w.seg; ++i) fold(sums + (((int64_t)w.b * nseg + i) * tiles + w.tile) * G::kSum, w, A, h);
 
   const T* const xp = static_cast<const T*>(kRev ? a.dy : a.x) + (int64_t)w.b * (kRev ? a.dy_sb : a.x_sb) + w.ch0;
   const T* const dp = static_cast<const T*>(a.dt) + (int64_t)w.b * a.dt_sb + w.ch0;
@@ -330,24 +484,24 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
   float bias[4], sum[4] = {};
 #pragma unroll
   for (int k = 0; k < 4; ++k) bias[k] = a.dt_bias != nullptr && c4 + k < w.nch ? a.dt_bias[w.ch0 + c4 + k] : 0.0f;
-  const float Dv = kOut && a.D != nullptr && w.own < w.nch ? a.D[w.ch0 + w.own] : 0.0f;
+  float Dv[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) Dv[k] = kOut && a.D != nullptr && c4 + k < w.nch ? a.D[w.ch0 + c4 + k] : 0.0f;
   const bool has_D = a.D != nullptr;
-  T* const yp = kOut ? static_cast<T*>(a.y) + (int64_t)w.b * a.seqlen * a.dim + w.ch0 + w.own : nullptr;
+  T* const yp = kOut ? static_cast<T*>(a.y) + (int64_t)w.b * a.seqlen * a.dim + w.ch0 + c4 : nullptr;
 
   const int count = (int)((end - begin + kT - 1) / kT);
   auto tile_start = [&](int i) { return begin + (kRev ? count - 1 - i : i) * kT; };
-  if (count > 0) stage_tile<T, G, kT, 3>(s.raw[0], src, stride, bc, bc_stride, tile_start(0), end, w.nch, a.dstate, vec.wide, vec.bc, lane);
+  if (count > 0) stage_tile<T, G, kT, 3>(s.raw[0], src, stride, bc, bc_stride, tile_start(0), end, w.nch, a.dstate, vec, lane);
   copy_commit();
   for (int i = 0; i < count; ++i) {
     const int t0 = tile_start(i);
     auto& raw = s.raw[i & 1];
-    if (i + 1 < count) stage_tile<T, G, kT, 3>(s.raw[(i + 1) & 1], src, stride, bc, bc_stride, tile_start(i + 1), end, w.nch, a.dstate, vec.wide, vec.bc, lane);
+    if (i + 1 < count) stage_tile<T, G, kT, 3>(s.raw[(i + 1) & 1], src, stride, bc, bc_stride, tile_start(i + 1), end, w.nch, a.dstate, vec, lane);
     copy_commit();
     copy_wait<1>();
     __syncwarp();
     if (t0 < live) {
-      if (kOut && a.checkpoints != nullptr && t0 > 0)
-        store_record<G>(a.checkpoints + (((int64_t)w.b * ((a.seqlen + kCkpt - 1) / kCkpt) + t0 / kCkpt) * tiles + w.tile) * kRec, lane, h);
 #pragma unroll
       for (int j = 0; j < kT / G::kRows; ++j) {
         const int t = j * G::kRows + row;
@@ -356,17 +510,13 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
         float4 zv;
         if (kRev && zp != nullptr) zv = quad(&raw.wide[2][t][c4]);
         float d[4], u[4];
+        deltas(dv, bias, a.dt_softplus, d);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const bool on = in && c4 + k < w.nch;
-          const float v = at(dv, k) + bias[k];
-          d[k] = on ? (a.dt_softplus ? softplus_series(v) : v) : 0.0f;
-          float g = at(xv, k);
-          if (kRev) {
-            if (zp != nullptr) g *= at(zv, k) * sigmoid_fast(at(zv, k));
-          } else {
-            g *= d[k];
-          }
+          float g = at(xv, k) * (kRev ? 1.0f : d[k]);
+          if (kRev && zp != nullptr) g *= at(zv, k) * sigmoid_fast(at(zv, k));
+          d[k] = on ? d[k] : 0.0f;
           u[k] = on ? g : 0.0f;
           sum[k] += d[k];
         }
@@ -375,61 +525,103 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
       }
       widen_bc<T, G, kT>(raw, s.bc, t0, min(live, end), a.dstate, lane);
       __syncwarp();
-#pragma unroll 4
-      for (int j = 0; j < kT; ++j) {
-        const int t = kRev ? kT - 1 - j : j;
-        float d[G::kCh], u[G::kCh], y[G::kCh];
-        f2 in2[G::kPairs], c2[G::kPairs];
-        load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
-        load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
-        load_pairs<G::kPairs>(&s.bc[kRev ? 1 : 0][t][w.q * kNp], in2);
-        if (kOut) load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
 #pragma unroll
-        for (int c = 0; c < G::kCh; ++c) {
-          const f2 dd = pack2(d[c], d[c]), uu = pack2(u[c], u[c]);
-          f2 acc = 0ull;
+      for (int half = 0; half < kT; half += kCkpt) {
+        const int todo = min(live, end) - t0;
+        if (half == 8 && todo > 8) {
+          float two[G::kCh], more[G::kCh];
+          load_channels<G::kCh>(&s.delta[3][w.cg * G::kCh], two);
+          load_channels<G::kCh>(&s.delta[11][w.cg * G::kCh], more);
 #pragma unroll
-          for (int p = 0; p < G::kPairs; ++p) {
-            const f2 e = exp2_pair(mul2(dd, A[c][p]));
-            if (kRev)
-              h[c][p] = mul2(e, fma2(in2[p], uu, h[c][p]));
-            else
-              h[c][p] = fma2(e, h[c][p], mul2(in2[p], uu));
-            if (kOut) acc = fma2(h[c][p], c2[p], acc);
-          }
-          if (kOut) {
-            float lo, hi;
-            unpack2(acc, lo, hi);
-            y[c] = lo + hi;
-          }
+          for (int c = 0; c < G::kCh; ++c) two[c] += more[c];
+          make_up<G>(two, (float)min(kT, todo), A, h);
         }
-        if (kOut) {
-          float v = own_channel<G::kCh>(y, w.q);
-          if (w.writes && t0 + t < end) {
-            if (has_D) v = fmaf(Dv, to_f(raw.wide[0][t][w.own]), v);
-            if (zp != nullptr) {
-              const float zv = to_f(raw.wide[2][t][w.own]);
-              v *= zv * sigmoid_fast(zv);
+        if (kOut && a.checkpoints != nullptr && half < todo && t0 + half > 0) store_kept(a, w, (t0 + half) / kCkpt, h);
+#pragma unroll 1
+        for (int j0 = half; j0 < half + kCkpt; j0 += 4) {
+        float own[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = kRev ? kT - 1 - j0 - j : j0 + j;
+          float d[G::kCh], u[G::kCh], y[G::kCh];
+          f2 in2[G::kPairs], c2[G::kPairs], e[G::kCh][G::kPairs];
+          load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
+          decays<G>(d, A, e);
+          load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
+          load_pairs<G::kPairs>(&s.bc[kRev ? 1 : 0][t][w.q * kNp], in2);
+          if (kOut) load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
+          if (kRev) {
+#pragma unroll
+            for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+              for (int p = 0; p < G::kPairs; ++p) h[c][p] = mul2(e[c][p], fma2(in2[p], pack2(u[c], u[c]), h[c][p]));
+          } else {
+            f2 acc[G::kCh];
+            advance<G>(e, u, in2, h);
+#pragma unroll
+            for (int p = 0; p < G::kPairs; ++p)
+#pragma unroll
+              for (int c = 0; c < G::kCh; ++c)
+                if (kOut) acc[c] = p == 0 ? mul2(h[c][0], c2[0]) : fma2(h[c][p], c2[p], acc[c]);
+#pragma unroll
+            for (int c = 0; c < G::kCh; ++c) {
+              float lo, hi;
+              if (kOut) unpack2(acc[c], lo, hi), y[c] = lo + hi;
             }
-            yp[(int64_t)(t0 + t) * a.dim] = from_f<T>(t0 + t < live ? v : 0.0f);
           }
+          if (kOut) own[j] = own_channel<G::kCh, G::kQ>(y, w.q);
+        }
+        if (kOut) {                                        // C . h takes the place of delta x, which these tokens no longer need
+          __syncwarp();
+          if (w.q % (G::kQ / G::kCh) == 0)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s.u[j0 + j][w.own] = own[j];
+        }
         }
       }
-    } else if (kOut && w.writes) {
-      for (int t = t0; t < min(t0 + kT, end); ++t) yp[(int64_t)t * a.dim] = from_f<T>(0.0f);
+      if (kOut) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kT / G::kRows; ++j) {
+          const int t = j * G::kRows + row;
+          const float4 yv = quad(&s.u[t][c4]), xv = quad(&raw.wide[0][t][c4]);
+          float4 zv;
+          if (zp != nullptr) zv = quad(&raw.wide[2][t][c4]);
+          float y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = at(yv, k);
+          if (has_D)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = fmaf(Dv[k], at(xv, k), y[k]);
+          if (zp != nullptr)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] *= at(zv, k) * sigmoid_fast(at(zv, k));
+          if (t0 + t >= live)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = 0.0f;
+          if (t0 + t < end) store_quad(yp + (int64_t)(t0 + t) * a.dim, y, w.nch - c4, vec.wide);
+        }
+      }
+    } else if (kOut) {
+      const float zero[4] = {};
+#pragma unroll
+      for (int j = 0; j < kT / G::kRows; ++j) {
+        const int t = t0 + j * G::kRows + row;
+        if (t < end) store_quad(yp + (int64_t)t * a.dim, zero, w.nch - c4, vec.wide);
+      }
     }
     __syncwarp();
   }
   if (kOut) {
     if (a.final_state != nullptr && w.seg == nseg - 1) store_state(a.final_state, a, w, h);
   } else {
-    float* rec = sums + (((int64_t)w.b * nseg + w.seg) * tiles + w.tile) * kSum;
+    float* rec = sums + (((int64_t)w.b * nseg + w.seg) * tiles + w.tile) * G::kSum;
     store_record<G>(rec, lane, h);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
       for (int o = G::kLanesRow; o < 32; o <<= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
-      if (row == 0) rec[kRec + c4 + k] = sum[k];
+      if (row == 0) rec[G::kRec + c4 + k] = sum[k];
     }
   }
 }
@@ -438,46 +630,97 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
 // With g_t = dy_t silu(z_t) and dh_t = C_t g_t + a_{t+1} dh_{t+1}:
 //   dC_t = sum_d g_t h_t, dB_t = sum_d dh_t delta_t x_t, dx_t = delta_t sum_n dh_t B_t + D g_t,
 //   ddelta_t = x_t sum_n dh_t B_t + sum_n A (dh_t a_t h_{t-1}), dA = sum_t delta_t (dh_t a_t h_{t-1}).
-// A warp walks its segment's chunks of 16 tokens from the last to the first.  A chunk's states come from the one kept at its
-// start: they are run forward once, and kept in shared memory before every fourth token; then four tokens at a time are run
-// forward again with decays and states in registers, and walked back.  (Running all 16 back from registers needs 512 of them;
-// keeping every state in shared memory moves 4 KB per token and warp through it.)
+// A warp walks its segment's chunks of eight tokens from the last to the first: forward once more from the state kept at the
+// chunk's start, then back.  The eight states of the way forward (128 floats a lane) wait in tensor memory, which nothing else here uses: a warp
+// reaches 32 of its lanes, one access moves a lane's 16 states, and 128 columns a CTA let four CTAs share an SM.  Kept in
+// registers they cost all occupancy, in shared memory 4 KB of traffic per token and warp.
 template <typename T, typename G>
 struct BwdWarpSmem {
   static constexpr int kT = kCkpt;
   static constexpr int kBuf = sizeof(T) == 2 ? 2 : 1;
   Raw<T, G, kT, 4> raw[kBuf];
   float delta[kT][G::kWc], u[kT][G::kWc], g[kT][G::kWc];
+  float inner[kT][G::kWc], through[kT][G::kWc], into[kT][G::kWc];
   float bc[2][kT][G::kN];
-  float keep[4][kRec];
   float part[kT][2][G::kN];
 };
 
-template <typename T, int kNp>
-__global__ void __launch_bounds__(32 * kBwdWarps)
+// a lane's 8 or 16 floats to and from its row of tensor memory
+template <typename G>
+__device__ __forceinline__ void tmem_keep(uint32_t at, const f2 (&h)[G::kCh][G::kPairs]) {
+  uint32_t r[16];
+#pragma unroll
+  for (int i = 0; i < G::kCh * G::kPairs; ++i) {
+    r[2 * i] = (uint32_t)h[i / G::kPairs][i % G::kPairs];
+    r[2 * i + 1] = (uint32_t)(h[i / G::kPairs][i % G::kPairs] >> 32);
+  }
+  if constexpr (G::kRec == 512) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15])
+                 : "memory");
+  } else {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  }
+}
+template <typename G>
+__device__ __forceinline__ void tmem_fetch(uint32_t at, uint32_t (&r)[16]) {
+  if constexpr (G::kRec == 512) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at)
+                 : "memory");
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(at)
+                 : "memory");
+  }
+}
+// waits for the fetch; its registers pass through here, so that nothing reads them before
+template <typename G>
+__device__ __forceinline__ void tmem_fetched(uint32_t (&r)[16], f2 (&h)[G::kCh][G::kPairs]) {
+  tc::tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < G::kCh * G::kPairs; ++i) {
+    asm volatile("" : "+r"(r[2 * i]), "+r"(r[2 * i + 1]));
+    h[i / G::kPairs][i % G::kPairs] = (f2)r[2 * i] | ((f2)r[2 * i + 1] << 32);
+  }
+}
+__device__ __forceinline__ void tmem_kept_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T, typename G>
+__global__ void __launch_bounds__(32 * kBwdWarps, 4)
 float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nseg, int seg_len, const float* sums, float* part_bc, float* part_grad,
                       Vec vec) {
-  using G = Geo<T, kNp>;
   using S = BwdWarpSmem<T, G>;
-  constexpr int kT = S::kT, kBuf = S::kBuf, kV = 2 * kNp;
+  constexpr int kT = S::kT, kBuf = S::kBuf, kNp = G::kNp, kStates = G::kCh * kNp, kColumns = kT * kStates;
   extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ uint32_t s_tmem;
   const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
   S& s = reinterpret_cast<S*>(dyn)[warp];
+  if (warp == 0) {
+    tc::tmem_alloc(&s_tmem, kColumns);
+    tc::tmem_relinquish();
+  }
+  __syncthreads();
+  const uint32_t tmem = s_tmem + ((uint32_t)warp << 21);        // the warp's 32 lanes of tensor memory
   const int cpg = (tpg + kBwdWarps - 1) / kBwdWarps, ctas = cpg * a.groups, tiles = tpg * a.groups;
   const int cta = (int)(blockIdx.x % ctas), rest = (int)(blockIdx.x / ctas);
   const int in_group = (cta % cpg) * kBwdWarps + warp;
   Place<G> w(a, tpg, rest / nseg, rest % nseg, (cta / cpg) * tpg + min(in_group, tpg - 1), lane);
-  if (in_group >= tpg) {                                 // a warp past the group's last tile adds zeros to its CTA's sums
-    w.nch = 0;
-    w.writes = false;
-  }
+  if (in_group >= tpg) w.nch = 0;                        // a warp past the group's last tile adds zeros to its CTA's sums
   const int live = live_tokens(a, w.b);
   const int begin = w.seg * seg_len, end = min(a.seqlen, begin + seg_len);
 
   f2 A[G::kCh][G::kPairs], carry[G::kCh][G::kPairs], dA[G::kCh][G::kPairs];
   load_A(a, w, A);
   load_state(a.d_final, a, w, carry);
-  for (int i = nseg - 1; i > w.seg; --i) fold(sums + (((int64_t)w.b * nseg + i) * tiles + w.tile) * kSum, w, A, carry);
+#pragma unroll 4
+  for (int i = nseg - 1; i > w.seg; --i) fold(sums + (((int64_t)w.b * nseg + i) * tiles + w.tile) * G::kSum, w, A, carry);
 #pragma unroll
   for (int c = 0; c < G::kCh; ++c)
 #pragma unroll
@@ -491,37 +734,35 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
   const T* const bc[2] = {static_cast<const T*>(a.Bm) + (int64_t)w.b * a.B_sb + (int64_t)w.group * a.B_sg,
                           static_cast<const T*>(a.Cm) + (int64_t)w.b * a.C_sb + (int64_t)w.group * a.C_sg};
   const int64_t bc_stride[2] = {a.B_sl, a.C_sl};
-  const bool has_z = a.z != nullptr;
+  const bool has_z = a.z != nullptr, has_D = a.D != nullptr;
   const int row = lane / G::kLanesRow, c4 = (lane % G::kLanesRow) * 4;
-  float bias[4];
+  float bias[4], Dv[4], dD[4] = {}, dbias[4] = {};
 #pragma unroll
-  for (int k = 0; k < 4; ++k) bias[k] = a.dt_bias != nullptr && c4 + k < w.nch ? a.dt_bias[w.ch0 + c4 + k] : 0.0f;
-  const bool has_own = w.own < w.nch, has_D = a.D != nullptr;
-  const float Dv = has_D && has_own ? a.D[w.ch0 + w.own] : 0.0f;
-  const float own_bias = a.dt_bias != nullptr && has_own ? a.dt_bias[w.ch0 + w.own] : 0.0f;
-  float dD = 0.0f, dbias = 0.0f;
-  T* const dxp = a.d_x != nullptr ? static_cast<T*>(a.d_x) + at_out + w.own : nullptr;
-  T* const ddp = a.d_dt != nullptr ? static_cast<T*>(a.d_dt) + at_out + w.own : nullptr;
-  T* const dzp = a.d_z != nullptr && has_z ? static_cast<T*>(a.d_z) + at_out + w.own : nullptr;
+  for (int k = 0; k < 4; ++k) {
+    bias[k] = a.dt_bias != nullptr && c4 + k < w.nch ? a.dt_bias[w.ch0 + c4 + k] : 0.0f;
+    Dv[k] = has_D && c4 + k < w.nch ? a.D[w.ch0 + c4 + k] : 0.0f;
+  }
+  T* const dxp = a.d_x != nullptr ? static_cast<T*>(a.d_x) + at_out + c4 : nullptr;
+  T* const ddp = a.d_dt != nullptr ? static_cast<T*>(a.d_dt) + at_out + c4 : nullptr;
+  T* const dzp = a.d_z != nullptr && has_z ? static_cast<T*>(a.d_z) + at_out + c4 : nullptr;
   float* const part = part_bc + ((int64_t)cta * a.batch + w.b) * a.seqlen * (2 * G::kN);
-  const int nck = (a.seqlen + kCkpt - 1) / kCkpt;
 
   const int first = begin / kT, last = (end + kT - 1) / kT - 1;
   // whole chunks past the sequence: zeros
   int chunk = last;
   for (; chunk >= first && chunk * kT >= live; --chunk) {
     const int lim = min(end, chunk * kT + kT);
-    for (int t = chunk * kT; t < lim; ++t)
-      if (w.writes) {
-        if (dxp != nullptr) dxp[(int64_t)t * a.dim] = from_f<T>(0.0f);
-        if (ddp != nullptr) ddp[(int64_t)t * a.dim] = from_f<T>(0.0f);
-        if (dzp != nullptr) dzp[(int64_t)t * a.dim] = from_f<T>(0.0f);
-      }
+    const float zero[4] = {};
+    for (int t = chunk * kT + row; t < lim; t += G::kRows) {
+      if (dxp != nullptr) store_quad(dxp + (int64_t)t * a.dim, zero, w.nch - c4, vec.wide);
+      if (ddp != nullptr) store_quad(ddp + (int64_t)t * a.dim, zero, w.nch - c4, vec.wide);
+      if (dzp != nullptr) store_quad(dzp + (int64_t)t * a.dim, zero, w.nch - c4, vec.wide);
+    }
     for (int e = (int)threadIdx.x; e < (lim - chunk * kT) * 2 * G::kN; e += 32 * kBwdWarps) part[(int64_t)chunk * kT * 2 * G::kN + e] = 0.0f;
   }
   const int top = chunk;
   if (kBuf == 2) {
-    if (top >= first) stage_tile<T, G, kT, 4>(s.raw[0], src, stride, bc, bc_stride, top * kT, end, w.nch, a.dstate, vec.wide, vec.bc, lane);
+    if (top >= first) stage_tile<T, G, kT, 4>(s.raw[0], src, stride, bc, bc_stride, top * kT, end, w.nch, a.dstate, vec, lane);
     copy_commit();
   }
   for (; chunk >= first; --chunk) {
@@ -529,11 +770,11 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
     auto& raw = s.raw[(top - chunk) % kBuf];
     if (kBuf == 2) {
       if (chunk > first)
-        stage_tile<T, G, kT, 4>(s.raw[(top - chunk + 1) % kBuf], src, stride, bc, bc_stride, t0 - kT, end, w.nch, a.dstate, vec.wide, vec.bc, lane);
+        stage_tile<T, G, kT, 4>(s.raw[(top - chunk + 1) % kBuf], src, stride, bc, bc_stride, t0 - kT, end, w.nch, a.dstate, vec, lane);
       copy_commit();
       copy_wait<1>();
     } else {
-      stage_tile<T, G, kT, 4>(raw, src, stride, bc, bc_stride, t0, end, w.nch, a.dstate, vec.wide, vec.bc, lane);
+      stage_tile<T, G, kT, 4>(raw, src, stride, bc, bc_stride, t0, end, w.nch, a.dstate, vec, lane);
       copy_commit();
       copy_wait<0>();
     }
@@ -541,25 +782,29 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
     if (chunk == 0)
       load_state(a.initial_state, a, w, h);
     else
-      load_record<G>(a.checkpoints + (((int64_t)w.b * nck + chunk) * tiles + w.tile) * kRec, lane, h);
+      load_kept(a, w, chunk, h);
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < kT / G::kRows; ++j) {
+    for (int j = 0; j < (kT + G::kRows - 1) / G::kRows; ++j) {
       const int t = j * G::kRows + row;
+      if (t >= kT) break;
       const bool in = t0 + t < lim;
       const float4 xv = quad(&raw.wide[0][t][c4]), dv = quad(&raw.wide[1][t][c4]), yv = quad(&raw.wide[3][t][c4]);
       float4 zv;
       if (has_z) zv = quad(&raw.wide[2][t][c4]);
       float d[4], u[4], g[4];
+      deltas(dv, bias, a.dt_softplus, d);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) g[k] = at(yv, k);
+      if (has_z)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) g[k] *= at(zv, k) * sigmoid_fast(at(zv, k));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const bool on = in && c4 + k < w.nch;
-        const float v = at(dv, k) + bias[k];
-        d[k] = on ? (a.dt_softplus ? softplus_series(v) : v) : 0.0f;
         u[k] = on ? d[k] * at(xv, k) : 0.0f;
-        float gg = at(yv, k);
-        if (has_z) gg *= at(zv, k) * sigmoid_fast(at(zv, k));
-        g[k] = on ? gg : 0.0f;
+        d[k] = on ? d[k] : 0.0f;
+        g[k] = on ? g[k] : 0.0f;
       }
       *reinterpret_cast<float4*>(&s.delta[t][c4]) = make_float4(d[0], d[1], d[2], d[3]);
       *reinterpret_cast<float4*>(&s.u[t][c4]) = make_float4(u[0], u[1], u[2], u[3]);
@@ -567,129 +812,140 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
     }
     widen_bc<T, G, kT>(raw, s.bc, t0, lim, a.dstate, lane);
     __syncwarp();
-    // states before every fourth token
-    store_record<G>(&s.keep[0][0], lane, h);
-#pragma unroll 1
-    for (int sub = 1; sub < 4; ++sub) {
+    // forward: C . h, and dC's sums over the warp's channels
+#pragma unroll 2
+    for (int t = 0; t < kT; ++t) {
+      float d[G::kCh], u[G::kCh], g[G::kCh], y[G::kCh], v[kNp];
+      f2 b2[G::kPairs], c2[G::kPairs], sC[G::kPairs], acc[G::kCh], e[G::kCh][G::kPairs];
+      load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
+      decays<G>(d, A, e);
+      load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
+      load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
+      load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
+      load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
+      tmem_keep<G>(tmem + t * kStates, h);
+      advance<G>(e, u, b2, h);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = (sub - 1) * 4 + j;
-        float d[G::kCh], u[G::kCh];
-        f2 b2[G::kPairs];
-        load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
-        load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
-        load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
+      for (int p = 0; p < G::kPairs; ++p)
 #pragma unroll
         for (int c = 0; c < G::kCh; ++c) {
-          const f2 dd = pack2(d[c], d[c]), uu = pack2(u[c], u[c]);
-#pragma unroll
-          for (int p = 0; p < G::kPairs; ++p) h[c][p] = fma2(exp2_pair(mul2(dd, A[c][p])), h[c][p], mul2(b2[p], uu));
+          acc[c] = p == 0 ? mul2(h[c][0], c2[0]) : fma2(h[c][p], c2[p], acc[c]);
+          sC[p] = c == 0 ? mul2(pack2(g[0], g[0]), h[0][p]) : fma2(pack2(g[c], g[c]), h[c][p], sC[p]);
         }
+#pragma unroll
+      for (int c = 0; c < G::kCh; ++c) {
+        float lo, hi;
+        unpack2(acc[c], lo, hi);
+        y[c] = lo + hi;
       }
-      store_record<G>(&s.keep[sub][0], lane, h);
+      const float own = own_channel<G::kCh, G::kQ>(y, w.q);
+      if (w.q % (G::kQ / G::kCh) == 0) s.inner[t][w.own] = own;
+#pragma unroll
+      for (int p = 0; p < G::kPairs; ++p) unpack2(sC[p], v[2 * p], v[2 * p + 1]);
+      over_groups<kNp, G::kQ>(v, lane, &s.part[t][1][w.q * kNp]);
     }
-#pragma unroll 1
-    for (int sub = 3; sub >= 0; --sub) {
-      f2 e[4][G::kCh][G::kPairs], hp[5][G::kCh][G::kPairs];
-      float inner[4];
-      load_record<G>(&s.keep[sub][0], lane, hp[0]);      // a lane reads what it wrote itself
+    tmem_kept_wait();
+    // and back
+#pragma unroll 2
+    for (int t = kT - 1; t >= 0; --t) {
+      float d[G::kCh], u[G::kCh], g[G::kCh], through[G::kCh], into[G::kCh], v[kNp];
+      f2 b2[G::kPairs], c2[G::kPairs], sB[G::kPairs], e[G::kCh][G::kPairs], dh[G::kCh][G::kPairs], thr[G::kCh], q2[G::kCh];
+      uint32_t kept[16];
+      tmem_fetch<G>(tmem + t * kStates, kept);
+      load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
+      decays<G>(d, A, e);
+      load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
+      load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
+      load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
+      load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = sub * 4 + j;
-        float d[G::kCh], u[G::kCh], y[G::kCh];
-        f2 b2[G::kPairs], c2[G::kPairs];
-        load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
-        load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
-        load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
-        load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
+      for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+        for (int p = 0; p < G::kPairs; ++p) dh[c][p] = fma2(c2[p], pack2(g[c], g[c]), carry[c][p]);
+#pragma unroll
+      for (int c = 0; c < G::kCh; ++c)
+#pragma unroll
+        for (int p = 0; p < G::kPairs; ++p) carry[c][p] = mul2(dh[c][p], e[c][p]);
+#pragma unroll
+      for (int p = 0; p < G::kPairs; ++p)
 #pragma unroll
         for (int c = 0; c < G::kCh; ++c) {
-          const f2 dd = pack2(d[c], d[c]), uu = pack2(u[c], u[c]);
-          f2 acc = 0ull;
-#pragma unroll
-          for (int p = 0; p < G::kPairs; ++p) {
-            e[j][c][p] = exp2_pair(mul2(dd, A[c][p]));
-            hp[j + 1][c][p] = fma2(e[j][c][p], hp[j][c][p], mul2(b2[p], uu));
-            acc = fma2(hp[j + 1][c][p], c2[p], acc);
-          }
-          float lo, hi;
-          unpack2(acc, lo, hi);
-          y[c] = lo + hi;
+          sB[p] = c == 0 ? mul2(pack2(u[0], u[0]), dh[0][p]) : fma2(pack2(u[c], u[c]), dh[c][p], sB[p]);
+          thr[c] = p == 0 ? mul2(dh[c][0], b2[0]) : fma2(dh[c][p], b2[p], thr[c]);
         }
-        inner[j] = has_z ? own_channel<G::kCh>(y, w.q) : 0.0f;
+      tmem_fetched<G>(kept, h);
+#pragma unroll
+      for (int p = 0; p < G::kPairs; ++p)
+#pragma unroll
+        for (int c = 0; c < G::kCh; ++c) {
+          dh[c][p] = mul2(carry[c][p], h[c][p]);
+          q2[c] = p == 0 ? mul2(dh[c][0], A[c][0]) : fma2(dh[c][p], A[c][p], q2[c]);
+          dA[c][p] = fma2(dh[c][p], pack2(d[c], d[c]), dA[c][p]);
+        }
+#pragma unroll
+      for (int c = 0; c < G::kCh; ++c) {
+        float lo, hi;
+        unpack2(thr[c], lo, hi);
+        through[c] = lo + hi;
+        unpack2(q2[c], lo, hi);
+        into[c] = lo + hi;
       }
 #pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        const int t = sub * 4 + j;
-        float d[G::kCh], u[G::kCh], g[G::kCh], through[G::kCh], into[G::kCh];
-        f2 b2[G::kPairs], c2[G::kPairs], sB[G::kPairs], sC[G::kPairs];
-        load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
-        load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
-        load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
-        load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
-        load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
+      for (int p = 0; p < G::kPairs; ++p) unpack2(sB[p], v[2 * p], v[2 * p + 1]);
+      over_groups<kNp, G::kQ>(v, lane, &s.part[t][0][w.q * kNp]);
+      const float own_through = own_channel<G::kCh, G::kQ>(through, w.q), own_into = own_channel<G::kCh, G::kQ>(into, w.q);
+      if (w.q % (G::kQ / G::kCh) == 0) {
+        s.through[t][w.own] = own_through;
+        s.into[t][w.own] = own_into;
+      }
+    }
+    if (chunk % 2 == 1) {                                // the middle of a tile of the forward pass
+      float two[G::kCh], more[G::kCh];
+      load_channels<G::kCh>(&s.delta[1][w.cg * G::kCh], two);
+      load_channels<G::kCh>(&s.delta[5][w.cg * G::kCh], more);
 #pragma unroll
-        for (int p = 0; p < G::kPairs; ++p) sB[p] = sC[p] = 0ull;
+      for (int c = 0; c < G::kCh; ++c) two[c] += more[c];
+      make_up<G>(two, (float)min(2 * kT, lim - t0 + kT), A, carry);
+    }
+    __syncwarp();
 #pragma unroll
-        for (int c = 0; c < G::kCh; ++c) {
-          const f2 dd = pack2(d[c], d[c]), uu = pack2(u[c], u[c]), gg = pack2(g[c], g[c]);
-          f2 thr = 0ull, q2 = 0ull;
+    for (int j = 0; j < (kT + G::kRows - 1) / G::kRows; ++j) {
+      const int t = j * G::kRows + row;
+      if (t >= kT) break;
+      const bool in = t0 + t < lim;
+      const float4 th = quad(&s.through[t][c4]), it = quad(&s.into[t][c4]), al = quad(&s.inner[t][c4]), dl = quad(&s.delta[t][c4]), gv = quad(&s.g[t][c4]);
+      const float4 xv = quad(&raw.wide[0][t][c4]), dv = quad(&raw.wide[1][t][c4]), yv = quad(&raw.wide[3][t][c4]);
+      float4 zv;
+      if (has_z) zv = quad(&raw.wide[2][t][c4]);
+      float dx[4], dd[4], dz[4], x[4], slope[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+      bool on[4];
+      if (a.dt_softplus)
 #pragma unroll
-          for (int p = 0; p < G::kPairs; ++p) {
-            const f2 dh = fma2(c2[p], gg, carry[c][p]);
-            sC[p] = fma2(gg, hp[j + 1][c][p], sC[p]);
-            sB[p] = fma2(uu, dh, sB[p]);
-            thr = fma2(dh, b2[p], thr);
-            carry[c][p] = mul2(dh, e[j][c][p]);
-            const f2 v = mul2(carry[c][p], hp[j][c][p]);
-            q2 = fma2(v, A[c][p], q2);
-            dA[c][p] = fma2(v, dd, dA[c][p]);
-          }
-          float lo, hi;
-          unpack2(thr, lo, hi);
-          through[c] = lo + hi;
-          unpack2(q2, lo, hi);
-          into[c] = lo + hi;
+        for (int k = 0; k < 4; ++k) slope[k] = sigmoid_fast(at(dv, k) + bias[k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        on[k] = in && c4 + k < w.nch;
+        x[k] = on[k] ? at(xv, k) : 0.0f;
+        dx[k] = fmaf(Dv[k], at(gv, k), at(th, k) * at(dl, k));
+        dd[k] = fmaf(at(th, k), x[k], at(it, k) * kLn2) * slope[k];
+        dd[k] = on[k] ? dd[k] : 0.0f;
+        dx[k] = on[k] ? dx[k] : 0.0f;
+        dD[k] = fmaf(at(gv, k), x[k], dD[k]);
+        dbias[k] += dd[k];
+      }
+      if (has_z)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float sig = sigmoid_fast(at(zv, k));
+          const float full = fmaf(Dv[k], x[k], at(al, k));
+          dz[k] = at(yv, k) * full * sig * fmaf(at(zv, k), 1.0f - sig, 1.0f);
+          dz[k] = on[k] ? dz[k] : 0.0f;
         }
-        // dB and dC of this token over the warp's channels: value i of a lane's 2 kNp is (B | C, state); eight lane groups
-        // halve the list three times
-        float v[kV];
-#pragma unroll
-        for (int p = 0; p < G::kPairs; ++p) {
-          unpack2(sB[p], v[2 * p], v[2 * p + 1]);
-          unpack2(sC[p], v[kNp + 2 * p], v[kNp + 2 * p + 1]);
-        }
-#pragma unroll
-        for (int half = kV / 2, bit = 16; bit >= 4; half /= 2, bit >>= 1) {
-          const bool up = lane & bit;
-#pragma unroll
-          for (int k = 0; k < half; ++k) v[k] = (up ? v[half + k] : v[k]) + __shfl_xor_sync(0xffffffffu, up ? v[k] : v[half + k], bit);
-        }
-        const int at0 = ((lane >> 4) & 1) * (kV / 2) + ((lane >> 3) & 1) * (kV / 4) + ((lane >> 2) & 1) * (kV / 8);
-#pragma unroll
-        for (int k = 0; k < kV / 8; ++k) s.part[t][(at0 + k) / kNp][w.q * kNp + (at0 + k) % kNp] = v[k];
-
-        const float own_through = own_channel<G::kCh>(through, w.q), own_into = own_channel<G::kCh>(into, w.q) * kLn2;
-        if (w.writes && t0 + t < end) {
-          const bool in = t0 + t < lim;
-          const float xv = to_f(raw.wide[0][t][w.own]), dl = s.delta[t][w.own], gv = s.g[t][w.own];
-          const float dx = fmaf(Dv, gv, own_through * dl);
-          float dd = fmaf(own_through, xv, own_into);
-          if (a.dt_softplus) dd *= sigmoid_fast(to_f(raw.wide[1][t][w.own]) + own_bias);
-          const int64_t o = (int64_t)(t0 + t) * a.dim;
-          if (in) {
-            dD = fmaf(gv, xv, dD);
-            dbias += dd;
-          }
-          if (dxp != nullptr) dxp[o] = from_f<T>(in ? dx : 0.0f);
-          if (ddp != nullptr) ddp[o] = from_f<T>(in ? dd : 0.0f);
-          if (dzp != nullptr) {
-            const float zv = to_f(raw.wide[2][t][w.own]), sig = sigmoid_fast(zv);
-            float all = inner[j];
-            if (has_D) all = fmaf(Dv, xv, all);
-            dzp[o] = from_f<T>(in ? to_f(raw.wide[3][t][w.own]) * all * sig * fmaf(zv, 1.0f - sig, 1.0f) : 0.0f);
-          }
-        }
+      if (t0 + t < end) {
+        const int64_t at_t = (int64_t)(t0 + t) * a.dim;
+        if (dxp != nullptr) store_quad(dxp + at_t, dx, w.nch - c4, vec.wide);
+        if (ddp != nullptr) store_quad(ddp + at_t, dd, w.nch - c4, vec.wide);
+        if (dzp != nullptr) store_quad(dzp + at_t, dz, w.nch - c4, vec.wide);
       }
     }
     // the CTA's channels together
@@ -704,14 +960,24 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
     __syncthreads();
   }
   if (w.nch > 0) {
-    float* rec = part_grad + (((int64_t)w.b * nseg + w.seg) * tiles + w.tile) * kGrad;
+    float* rec = part_grad + (((int64_t)w.b * nseg + w.seg) * tiles + w.tile) * G::kGrad;
     store_record<G>(rec, lane, dA);
-    if (w.writes) {
-      rec[kRec + w.own] = dD;
-      rec[kRec + 32 + w.own] = dbias;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int o = G::kLanesRow; o < 32; o <<= 1) {
+        dD[k] += __shfl_xor_sync(0xffffffffu, dD[k], o);
+        dbias[k] += __shfl_xor_sync(0xffffffffu, dbias[k], o);
+      }
+      if (row == 0) {
+        rec[G::kRec + c4 + k] = dD[k];
+        rec[G::kRec + 32 + c4 + k] = dbias[k];
+      }
     }
     if (a.d_initial != nullptr && w.seg == 0) store_state(a.d_initial, a, w, carry);
   }
+  __syncthreads();
+  if (warp == 0) tc::tmem_dealloc(s_tmem, kColumns);
 }
 
 // dB and dC: the CTAs' sums added up in their order
@@ -729,15 +995,15 @@ __global__ void __launch_bounds__(256) float_scan_bc_kernel(const __grid_constan
 }
 
 // dA, dD, d_bias: summed over sequences and segments in their order
-template <int kNp>
-__global__ void __launch_bounds__(kGrad) float_scan_param_kernel(const __grid_constant__ qb_float_scan_args a, const float* part, int tpg, int runs) {
-  using G = Geo<float, kNp>;
+template <typename G>
+__global__ void __launch_bounds__(G::kGrad) float_scan_param_kernel(const __grid_constant__ qb_float_scan_args a, const float* part, int tpg, int runs) {
+  constexpr int kRec = G::kRec, kGrad = G::kGrad, kNp = G::kNp;
   const int tiles = tpg * a.groups, tile = (int)blockIdx.x, i = (int)threadIdx.x;
   const int per = a.dim / a.groups, c0 = (tile % tpg) * G::kWc, ch0 = tile / tpg * per + c0, nch = min(G::kWc, per - c0);
   const bool is_A = i < kRec;
   // a record's float4 k of lane l holds the values 4 k .. 4 k + 3 of that lane, value = channel of the lane * kNp + state
   const int l = i / 4 % 32, v = i / 128 * 4 + i % 4;
-  const int ch = is_A ? (l >> 2) * G::kCh + v / kNp : (i - kRec) % 32, n = is_A ? (l & 3) * kNp + v % kNp : 0;
+  const int ch = is_A ? l / G::kQ * G::kCh + v / kNp : (i - kRec) % 32, n = is_A ? l % G::kQ * kNp + v % kNp : 0;
   if (ch >= nch || (is_A && n >= a.dstate)) return;
   const float* p = part + (int64_t)tile * kGrad + i;
   float sum = 0.0f;
@@ -778,12 +1044,15 @@ __global__ void __launch_bounds__(128) float_update_kernel(const __grid_constant
   }
   const float x = to_f(static_cast<const T*>(a.x)[b * a.x_sb + d]);
   float dl = to_f(static_cast<const T*>(a.dt)[b * a.dt_sb + d]) + (a.dt_bias != nullptr ? a.dt_bias[d] : 0.0f);
-  if (a.dt_softplus) dl = softplus_series(dl);
+  if (a.dt_softplus) {
+    float twin = dl;
+    softplus_series(dl, twin);
+  }
   const float u = dl * x;
   float y = 0.0f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    h[k] = fmaf(fast_exp2(dl * A[k]), h[k], u * B[k]);
+    h[k] = fmaf(exp2_series(dl * A[k]), h[k], u * B[k]);   // one decay a call: see make_up()
     y = fmaf(h[k], C[k], y);
   }
 #pragma unroll
@@ -808,39 +1077,80 @@ __global__ void __launch_bounds__(128) float_update_kernel(const __grid_constant
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
+// How the work is dealt out.
 struct Plan {
-  int np, wc, tpg, tiles, nseg, seg_len;
+  int np, ch, q;                           // Geo
+  int tpg, tiles, nseg, seg_len;
+  int rec() const { return 32 * np * ch; }
+  int wide() const { return np * q; }
 };
-Plan plan_of(int batch, int seqlen, int dim, int groups, int dstate) {
-  Plan p;
-  p.np = dstate <= 16 ? 4 : dstate <= 32 ? 8 : 16;
-  p.wc = 128 / p.np;
-  p.tpg = (int)ceil_div(dim / groups, p.wc);
+constexpr int kMinSeg = 64;                // tokens of a segment, at least
+constexpr int kMaxSegs = 32;               // a segment folds the summaries of all on its one side
+
+Plan share_of(int batch, int dim, int groups, int np, int ch, int q) {
+  Plan p{np, ch, q, 0, 0, 1, 0};
+  p.tpg = (int)ceil_div(dim / groups, 32 / q * ch);
   p.tiles = p.tpg * groups;
-  p.nseg = 1;
-  p.seg_len = std::max(seqlen, 1);
-  (void)batch;
   return p;
 }
-int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-int64_t sums_bytes(const Plan& p, int64_t batch) { return p.nseg > 1 ? align256(batch * p.nseg * p.tiles * kSum * (int64_t)sizeof(float)) : 0; }
-int64_t part_bytes(const Plan& p, int64_t batch, int64_t seqlen, int groups) {
-  return align256(ceil_div(p.tpg, kBwdWarps) * groups * batch * seqlen * 8 * p.np * (int64_t)sizeof(float));
+void cut(Plan& p, int seqlen, int64_t want) {
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, kMaxSegs), seqlen / kMinSeg));
+  p.seg_len = (int)std::max<int64_t>(16, ceil_div(ceil_div(seqlen, n), 16) * 16);
+  p.nseg = (int)std::max<int64_t>(1, ceil_div(seqlen, p.seg_len));
 }
-int64_t grad_bytes(const Plan& p, int64_t batch) { return align256(batch * p.nseg * p.tiles * kGrad * (int64_t)sizeof(float)); }
+// Forward.  Eight states a lane: sixteen take fewer instructions but leave too few warps on an SM to hide each one's latencies
+// (8 x 1024 tokens of 5120 channels: 389 us against 440).  Rows that put fewer than eight warps on an SM are cut into segments, which are
+// walked twice (512 tokens of 1536 channels: 28 us, in one piece 68; 4 x 2048 of 5120, nine warps: 515, cut in four 532).  A
+// short sequence cannot be cut often enough and takes four states a lane.
+Plan plan_fwd(int batch, int seqlen, int dim, int groups, int dstate) {
+  Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 1, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 1, 4) : share_of(batch, dim, groups, 16, 1, 4);
+  const int64_t sms = sm_count();
+  if (dstate <= 16 && (int64_t)batch * p.tiles < 8 * sms && (int64_t)batch * p.tiles * std::max(1, seqlen / kMinSeg) < 12 * sms)
+    p = share_of(batch, dim, groups, 4, 1, 4);
+  const int64_t warps = std::max<int64_t>(1, (int64_t)batch * p.tiles);
+  cut(p, seqlen, warps >= 8 * sms ? 1 : ceil_div(32 * sms, warps));
+  return p;
+}
+// Backward: sixteen states a lane where that gives every SM four warps, else eight; and as many segments as make the number of
+// waves of resident CTAs (four an SM) times a segment's length smallest.  A segment's summary costs a quarter of its walk.  8 x 1024
+// tokens of 5120 channels: 1.26 ms in twelve segments, 1.54 in one piece.
+Plan plan_bwd(int batch, int seqlen, int dim, int groups, int dstate) {
+  const int64_t sms = sm_count();
+  Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 2, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 2, 4) : share_of(batch, dim, groups, 16, 1, 4);
+  if (p.ch == 2 && (int64_t)batch * p.tiles < 4 * sms) p = share_of(batch, dim, groups, 8, 1, p.q);
+  const int64_t ctas = std::max<int64_t>(1, (int64_t)batch * groups * ceil_div(p.tpg, kBwdWarps)), slots = 4 * sms;
+  int64_t best = 1;
+  double least = 0.0;
+  for (int64_t n = 1; n <= std::min<int64_t>(24, std::max(1, seqlen / kMinSeg)); ++n) {
+    const double cost = (double)ceil_div(ctas * n, slots) / n * (1.0 + 0.25 * (n - 1) / n);
+    if (n == 1 || cost < least) { least = cost; best = n; }
+  }
+  cut(p, seqlen, best);
+  return p;
+}
+Plan plan_of(int batch, int seqlen, int dim, int groups, int dstate, bool backward) {
+  return backward ? plan_bwd(batch, seqlen, dim, groups, dstate) : plan_fwd(batch, seqlen, dim, groups, dstate);
+}
+int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+int64_t sums_bytes(const Plan& p, int64_t batch) { return p.nseg > 1 ? align256(batch * p.nseg * p.tiles * (p.rec() + 32) * (int64_t)sizeof(float)) : 0; }
+int64_t part_bytes(const Plan& p, int64_t batch, int64_t seqlen, int groups) {
+  return align256(ceil_div(p.tpg, kBwdWarps) * groups * batch * seqlen * 2 * p.wide() * (int64_t)sizeof(float));
+}
+int64_t grad_bytes(const Plan& p, int64_t batch) { return align256(batch * p.nseg * p.tiles * (p.rec() + 64) * (int64_t)sizeof(float)); }
 
 bool sizes_ok(int64_t batch, int64_t seqlen, int64_t dim, int64_t groups, int64_t dstate) {
   return batch >= 0 && seqlen >= 0 && dim > 0 && groups > 0 && dim % groups == 0 && dstate >= 1 && dstate <= 64;
 }
 bool quads(const void* p, int64_t s1, int64_t s2, size_t size) { return p == nullptr || (aligned(p, 4 * size) && s1 % 4 == 0 && s2 % 4 == 0); }
 
-int check_scan(const qb_float_scan_args* a, const char* who) {
+int check_scan(const qb_float_scan_args* a, bool backward) {
+  const char* who = backward ? "float_scan_bwd" : "float_scan_fwd";
   QB_REQUIRE(a != nullptr && a->x && a->dt && a->Bm && a->Cm && a->A, QB_ERR_INVALID_ARG, "%s: null pointer", who);
   QB_REQUIRE(a->dstate >= 1 && a->dstate <= 64, QB_ERR_INVALID_ARG, "%s: dstate must be 1 to 64, got %d", who, a->dstate);
   QB_REQUIRE(a->batch >= 0 && a->seqlen >= 0 && a->dim > 0 && a->groups > 0, QB_ERR_INVALID_ARG, "%s: bad shape", who);
   QB_REQUIRE(a->dim % a->groups == 0, QB_ERR_INVALID_ARG, "%s: dim = %d is not divisible by groups = %d", who, a->dim, a->groups);
   QB_REQUIRE(a->dtype >= 0 && a->dtype <= 2, QB_ERR_INVALID_ARG, "%s: unsupported type", who);
-  const Plan p = plan_of(a->batch, a->seqlen, a->dim, a->groups, a->dstate);
+  const Plan p = plan_of(a->batch, a->seqlen, a->dim, a->groups, a->dstate, backward);
   QB_REQUIRE((int64_t)a->batch * p.nseg * p.tiles < (1ll << 31), QB_ERR_TOO_LARGE, "%s: batch and dim are too large", who);
   return QB_OK;
 }
@@ -852,55 +1162,54 @@ Vec vec_of(const qb_float_scan_args& a, bool backward) {
   return Vec{wide, bc};
 }
 
-template <typename T, int kNp, int kMode>
+template <typename T, typename G, int kMode>
 int launch_scan(const qb_float_scan_args& a, const Plan& p, float* sums, Vec vec, cudaStream_t st) {
-  const size_t smem = sizeof(FwdSmem<T, Geo<T, kNp>>);
+  const size_t smem = sizeof(FwdSmem<T, G>);
   static PerDeviceOnce attr;
   const int rc = attr.run([&]() -> int {
-    QB_CUDA_OK(cudaFuncSetAttribute(float_scan_kernel<T, kNp, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    QB_CUDA_OK(cudaFuncSetAttribute(float_scan_kernel<T, G, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     return QB_OK;
   });
   if (rc != QB_OK) return rc;
   const int64_t grid = (int64_t)a.batch * (p.nseg - (kMode == 0 ? 0 : 1)) * p.tiles;
-  float_scan_kernel<T, kNp, kMode><<<(unsigned)grid, 32, smem, st>>>(a, p.tpg, p.nseg, p.seg_len, sums, vec);
+  float_scan_kernel<T, G, kMode><<<(unsigned)grid, 32, smem, st>>>(a, p.tpg, p.nseg, p.seg_len, sums, vec);
   QB_LAUNCH_OK("float_scan_kernel");
   return QB_OK;
 }
 
-template <typename T, int kNp>
+template <typename T, typename G>
 int run_fwd(const qb_float_scan_args& a, const Plan& p, cudaStream_t st) {
   float* sums = static_cast<float*>(a.workspace);
   const Vec vec = vec_of(a, false);
   if (p.nseg > 1) {
-    const int rc = launch_scan<T, kNp, 1>(a, p, sums, vec, st);
+    const int rc = launch_scan<T, G, 1>(a, p, sums, vec, st);
     if (rc != QB_OK) return rc;
   }
-  return launch_scan<T, kNp, 0>(a, p, sums, vec, st);
+  return launch_scan<T, G, 0>(a, p, sums, vec, st);
 }
 
-template <typename T, int kNp>
+template <typename T, typename G>
 int run_bwd(const qb_float_scan_args& a, const Plan& p, cudaStream_t st) {
-  using G = Geo<T, kNp>;
   unsigned char* ws = static_cast<unsigned char*>(a.workspace);
   float* sums = reinterpret_cast<float*>(ws);
   float* part = reinterpret_cast<float*>(ws + sums_bytes(p, a.batch));
   float* grad = reinterpret_cast<float*>(ws + sums_bytes(p, a.batch) + part_bytes(p, a.batch, a.seqlen, a.groups));
   const Vec vec = vec_of(a, true);
   if (p.nseg > 1 && a.batch > 0) {
-    const int rc = launch_scan<T, kNp, 2>(a, p, sums, vec, st);
+    const int rc = launch_scan<T, G, 2>(a, p, sums, vec, st);
     if (rc != QB_OK) return rc;
   }
   const size_t smem = sizeof(BwdWarpSmem<T, G>) * kBwdWarps;
   static PerDeviceOnce attr;
   const int rc = attr.run([&]() -> int {
-    QB_CUDA_OK(cudaFuncSetAttribute(float_scan_bwd_kernel<T, kNp>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    QB_CUDA_OK(cudaFuncSetAttribute(float_scan_bwd_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     return QB_OK;
   });
   if (rc != QB_OK) return rc;
   const int cpg = (int)ceil_div(p.tpg, kBwdWarps);
   if (a.batch > 0) {
     const int64_t grid = (int64_t)a.batch * p.nseg * cpg * a.groups;
-    float_scan_bwd_kernel<T, kNp><<<(unsigned)grid, 32 * kBwdWarps, smem, st>>>(a, p.tpg, p.nseg, p.seg_len, sums, part, grad, vec);
+    float_scan_bwd_kernel<T, G><<<(unsigned)grid, 32 * kBwdWarps, smem, st>>>(a, p.tpg, p.nseg, p.seg_len, sums, part, grad, vec);
     QB_LAUNCH_OK("float_scan_bwd_kernel");
   }
   const int64_t cells = (int64_t)a.batch * a.seqlen * a.groups * 2 * G::kN;
@@ -909,7 +1218,7 @@ int run_bwd(const qb_float_scan_args& a, const Plan& p, cudaStream_t st) {
     QB_LAUNCH_OK("float_scan_bc_kernel");
   }
   if (a.d_A != nullptr || a.d_D != nullptr || a.d_bias != nullptr) {
-    float_scan_param_kernel<kNp><<<(unsigned)p.tiles, kGrad, 0, st>>>(a, grad, p.tpg, a.batch * p.nseg);
+    float_scan_param_kernel<G><<<(unsigned)p.tiles, G::kGrad, 0, st>>>(a, grad, p.tpg, a.batch * p.nseg);
     QB_LAUNCH_OK("float_scan_param_kernel");
   }
   return QB_OK;
@@ -919,6 +1228,18 @@ template <typename F>
 int by_type(int dtype, F f) {
   return dtype == 0 ? f(float{}) : dtype == 1 ? f(__half{}) : f(__nv_bfloat16{});
 }
+template <typename F>
+int by_share_fwd(const Plan& p, F f) {
+  if (p.np == 4) return f(Geo<4, 1, 4>{});
+  if (p.np == 8) return p.q == 2 ? f(Geo<8, 1, 2>{}) : f(Geo<8, 1, 4>{});
+  return f(Geo<16, 1, 4>{});
+}
+template <typename F>
+int by_share_bwd(const Plan& p, F f) {
+  if (p.q == 2) return p.ch == 2 ? f(Geo<8, 2, 2>{}) : f(Geo<8, 1, 2>{});
+  if (p.np == 8) return p.ch == 2 ? f(Geo<8, 2, 4>{}) : f(Geo<8, 1, 4>{});
+  return f(Geo<16, 1, 4>{});
+}
 
 }  // namespace
 }  // namespace qb
@@ -927,21 +1248,21 @@ using namespace qb;
 
 extern "C" int64_t qb_float_scan_checkpoint_bytes(int32_t batch, int32_t seqlen, int32_t dim, int32_t groups, int32_t dstate) {
   if (!sizes_ok(batch, seqlen, dim, groups, dstate)) return -1;
-  return (int64_t)batch * ceil_div(seqlen, kCkpt) * plan_of(batch, seqlen, dim, groups, dstate).tiles * kRec * (int64_t)sizeof(float);
+  return (int64_t)batch * ceil_div(seqlen, kCkpt) * dim * (dstate <= 16 ? 16 : dstate <= 32 ? 32 : 64) * (int64_t)sizeof(float);
 }
 
 extern "C" int64_t qb_float_scan_workspace_bytes(int32_t batch, int32_t seqlen, int32_t dim, int32_t groups, int32_t dstate, int32_t backward) {
   if (!sizes_ok(batch, seqlen, dim, groups, dstate)) return -1;
-  const Plan p = plan_of(batch, seqlen, dim, groups, dstate);
+  const Plan p = plan_of(batch, seqlen, dim, groups, dstate, backward != 0);
   return sums_bytes(p, batch) + (backward ? part_bytes(p, batch, seqlen, groups) + grad_bytes(p, batch) : 0);
 }
 
 extern "C" int qb_float_scan_fwd(const qb_float_scan_args* a, void* stream) {
-  const int rc = check_scan(a, "float_scan_fwd");
+  const int rc = check_scan(a, false);
   if (rc != QB_OK) return rc;
   QB_REQUIRE(a->y != nullptr || (int64_t)a->batch * a->seqlen == 0, QB_ERR_INVALID_ARG, "float_scan_fwd: null output");
   if (a->batch == 0) return QB_OK;
-  const Plan p = plan_of(a->batch, a->seqlen, a->dim, a->groups, a->dstate);
+  const Plan p = plan_of(a->batch, a->seqlen, a->dim, a->groups, a->dstate, false);
   const int64_t need = sums_bytes(p, a->batch);
   QB_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need && aligned(a->workspace, 16)), QB_ERR_INVALID_ARG,
              "float_scan_fwd: the workspace must have %lld bytes, 16-byte aligned", (long long)need);
@@ -949,23 +1270,23 @@ extern "C" int qb_float_scan_fwd(const qb_float_scan_args* a, void* stream) {
   return by_type(a->dtype, [&](auto t) -> int {
     using T = decltype(t);
     cudaStream_t st = (cudaStream_t)stream;
-    return p.np == 4 ? run_fwd<T, 4>(*a, p, st) : p.np == 8 ? run_fwd<T, 8>(*a, p, st) : run_fwd<T, 16>(*a, p, st);
+    return by_share_fwd(p, [&](auto g) -> int { return run_fwd<T, decltype(g)>(*a, p, st); });
   });
 }
 
 extern "C" int qb_float_scan_bwd(const qb_float_scan_args* a, void* stream) {
-  const int rc = check_scan(a, "float_scan_bwd");
+  const int rc = check_scan(a, true);
   if (rc != QB_OK) return rc;
   QB_REQUIRE((a->dy != nullptr && a->checkpoints != nullptr) || (int64_t)a->batch * a->seqlen == 0, QB_ERR_INVALID_ARG, "float_scan_bwd: dy and checkpoints are needed");
   QB_REQUIRE(aligned(a->checkpoints, 16), QB_ERR_INVALID_ARG, "float_scan_bwd: checkpoints must be 16-byte aligned");
-  const Plan p = plan_of(a->batch, a->seqlen, a->dim, a->groups, a->dstate);
+  const Plan p = plan_of(a->batch, a->seqlen, a->dim, a->groups, a->dstate, true);
   const int64_t need = qb_float_scan_workspace_bytes(a->batch, a->seqlen, a->dim, a->groups, a->dstate, 1);
   QB_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need && aligned(a->workspace, 16)), QB_ERR_INVALID_ARG,
              "float_scan_bwd: the workspace must have %lld bytes, 16-byte aligned", (long long)need);
   return by_type(a->dtype, [&](auto t) -> int {
     using T = decltype(t);
     cudaStream_t st = (cudaStream_t)stream;
-    return p.np == 4 ? run_bwd<T, 4>(*a, p, st) : p.np == 8 ? run_bwd<T, 8>(*a, p, st) : run_bwd<T, 16>(*a, p, st);
+    return by_share_bwd(p, [&](auto g) -> int { return run_bwd<T, decltype(g)>(*a, p, st); });
   });
 }
 

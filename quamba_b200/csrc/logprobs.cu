@@ -1,7 +1,17 @@
 // Log probabilities of given tokens, entropy and likeliest alternatives from rows of logits, and their gradient (sm_100a).
 //
-// One pass over a row with a running maximum m and, relative to it, s = sum exp(x - m) and w = sum exp(x - m) (x - m):
-//   logprob = (x_target - m) - log s, entropy = log s - w / s.
+// Forward: one pass over a row in 16-byte pieces.  With t = (x - m) log2 e for a reference m of the thread's own (raised when a
+// value passes it by far), s = sum 2^t and w = sum t 2^t give
+//   logprob = (x_target - m) - log2 s ln 2,   entropy = (log2 s - w / s) ln 2,
+// in packed fp32 pairs: 3 to 4 issue slots and one MUFU result per value, against the 11 slots and 1.4 results that a 2-byte value
+// leaves at the memory's speed.  Many rows take a CTA each; few rows a cluster of up to eight, whose parts are joined over
+// distributed shared memory.
+//
+// Alternatives in the same pass.  Of the first piece of every thread the maxima of 128 groups are ranked: the top_k-th of them is a bound
+// that at least top_k values reach, so what is below it never counts again.  Values that reach it are listed (some hundreds), and
+// the list is ranked at the end by (value, column).  A list that runs over (long plateaus of equal values, rows that rise to
+// the end) sends the row's part to top_k searches for the largest key below the last.
+//
 // Bound by the row's bytes: read once forward; read and written once backward.
 #include <algorithm>
 #include "common.cuh"
@@ -13,13 +23,17 @@ int* device_status_ptr();
 namespace {
 
 constexpr int kStatusTarget = 502;       // keep in step with qb_read_device_status (lib.cu)
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kFar = -1.0e4f;           // stands for everything below it where it is multiplied by an exponential that is zero there
+constexpr int kMaxCluster = 8;
+constexpr int kGroups = 128;             // groups of threads whose first maxima are ranked
+constexpr int kList = 2048;              // candidates listed per CTA
+constexpr int kTop = QB_LOGPROBS_MAX_TOP;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kFar = -1.0e4f;           // stands for everything below it where it is multiplied by a power that is zero there
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7fc00000); }
 
-template <typename T> struct Wide { static constexpr int kN = 16 / sizeof(T); T v[kN]; };
+template <typename T> struct Wide { static constexpr int kN = 16 / sizeof(T); __align__(16) T v[kN]; };
 __device__ __forceinline__ float val(float v) { return v; }
 __device__ __forceinline__ float val(__half v) { return __half2float(v); }
 __device__ __forceinline__ float val(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -34,130 +48,309 @@ __device__ __forceinline__ Wide<T> load16(const T* p) {
   *reinterpret_cast<uint4*>(r.v) = *reinterpret_cast<const uint4*>(p);
   return r;
 }
+// the largest of a piece (a NaN beside numbers is passed over: it stays in the sums)
+__device__ __forceinline__ float largest(const Wide<float>& r) { return fmaxf(fmaxf(r.v[0], r.v[1]), fmaxf(r.v[2], r.v[3])); }
+__device__ __forceinline__ float largest(const Wide<__half>& r) {
+  const __half2* h = reinterpret_cast<const __half2*>(r.v);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return __half2float(__hmax(__low2half(m), __high2half(m)));
+}
+__device__ __forceinline__ float largest(const Wide<__nv_bfloat16>& r) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(r.v);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m)));
+}
 
-struct Stats { float m, s, w; };
-// m may be below the largest value by up to kSlack without harm: s and w are floats with exponents to spare
+struct Stats { float m, s, w; };         // m: the reference, -inf before the first number
+// a headroom of e^kSlack costs s and w nothing: they are floats with exponents to spare
 constexpr float kSlack = 16.0f;
 __device__ __forceinline__ void raise(Stats& a, float m) {
   if (a.m != neg_inf()) {
-    const float d = fmaxf(a.m - m, kFar), f = __expf(d);
+    const float d = fmaxf((a.m - m) * kLog2e, kFar), f = fast_exp2(d);
     a.w = (a.w + a.s * d) * f;
     a.s *= f;
   }
   a.m = m;
 }
-template <int kN>
-__device__ __forceinline__ void add(Stats& a, const float (&x)[kN]) {
-  float top = x[0];
-#pragma unroll
-  for (int k = 1; k < kN; ++k) top = fmaxf(top, x[k]);
-  if (top > a.m + kSlack) raise(a, top);              // always when a.m is still -inf and top is not
-  const float m = a.m == neg_inf() ? 0.0f : a.m;
-#pragma unroll
-  for (int k = 0; k < kN; ++k) {
-    const float d = x[k] - m, e = fast_exp2(d * kLog2e);   // NaN stays NaN
-    a.s += e;
-    a.w = fmaf(e, fmaxf(d, kFar), a.w);
-  }
-}
-__device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
-  // by the larger maximum; an empty side (m = -inf) may still hold a NaN in s
-  const float m = fmaxf(a.m, b.m);
-  if (m == neg_inf()) return Stats{m, a.s + b.s, a.w + b.w};
-  Stats x = a, y = b;
-  if (x.m != m) { if (x.m == neg_inf()) x = Stats{m, a.s, a.w}; else raise(x, m); }
-  if (y.m != m) { if (y.m == neg_inf()) y = Stats{m, b.s, b.w}; else raise(y, m); }
+__device__ __forceinline__ Stats join(Stats x, Stats y) {
+  const float m = fmaxf(x.m, y.m);
+  if (x.m != m) raise(x, m);               // a side without numbers (m = -inf) has s = w = 0, or a NaN
+  if (y.m != m) raise(y, m);
   return Stats{m, x.s + y.s, x.w + y.w};
+}
+template <bool kEntropy>
+__device__ __forceinline__ void add_one(Stats& a, float x) {
+  if (x > a.m + kSlack) raise(a, x);
+  const float t = (x - (a.m == neg_inf() ? 0.0f : a.m)) * kLog2e, e = fast_exp2(t);
+  a.s += e;
+  if (kEntropy) a.w = fmaf(e, fmaxf(t, kFar), a.w);
+}
+template <bool kEntropy, typename T>
+__device__ __forceinline__ void add_piece(Stats& a, f2& s2, f2& w2, const Wide<T>& r, float top) {
+  if (top > a.m + kSlack) {                // the pairs' sums go into the scalar ones first: they are relative to the old reference
+    float x, y;
+    unpack2(s2, x, y);
+    a.s += x + y;
+    unpack2(w2, x, y);
+    a.w += x + y;
+    s2 = w2 = 0ull;
+    raise(a, top);
+  }
+  const float m = a.m == neg_inf() ? 0.0f : -a.m;
+  const f2 mm = pack2(m, m), l2 = pack2(kLog2e, kLog2e);
+#pragma unroll
+  for (int k = 0; k < Wide<T>::kN; k += 2) {
+    float x, y;
+    const f2 t = mul2(add2(pack2(val(r.v[k]), val(r.v[k + 1])), mm), l2);   // not one fma: x log2 e may be out of range
+    unpack2(t, x, y);
+    const f2 e = pack2(fast_exp2(x), fast_exp2(y));          // NaN stays NaN
+    s2 = add2(s2, e);
+    if (kEntropy) w2 = fma2(e, pack2(fmaxf(x, kFar), fmaxf(y, kFar)), w2);
+  }
 }
 
 // order-preserving key of (value, column): larger value first, then lower column; -0 counts as 0
-__device__ __forceinline__ uint64_t key_of(float v, uint32_t col) {
+__device__ __forceinline__ uint32_t rank_of(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);
-  return ((uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32) | (0xffffffffu - col);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t col) { return ((uint64_t)rank_of(v) << 32) | (0xffffffffu - col); }
 __device__ __forceinline__ float value_of(uint64_t key) {
   const uint32_t u = (uint32_t)(key >> 32);
   return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
 }
 __device__ __forceinline__ uint32_t column_of(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// calls f(values, first column) over a row in 16-byte pieces, and over what lies before and after them one by one
-template <typename T, typename F>
-__device__ __forceinline__ void walk_row(const T* row, int vocab, int thread, int threads, F f) {
-  constexpr int kN = Wide<T>::kN;
-  const int head = min(vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)));
-  const int body = (vocab - head) / kN;
-  for (int i = thread; i < body; i += threads) {
-    const Wide<T> r = load16(row + head + i * kN);
-    float x[kN];
-#pragma unroll
-    for (int k = 0; k < kN; ++k) x[k] = val(r.v[k]);
-    f(x, head + i * kN);
+// A part of a row: columns before the first 16-byte boundary, pieces, columns after the last.
+template <typename T>
+struct Part {
+  const T* row;
+  int begin, head, body, rest;             // columns [begin, begin + head), body pieces, rest columns in all besides the pieces
+  __device__ __forceinline__ Part(const T* row_, int from, int to) : row(row_), begin(from) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + from) & 15;
+    head = min(to - from, (int)(((16 - at) & 15) / sizeof(T)));
+    body = (to - from - head) / Wide<T>::kN;
+    rest = to - from - body * Wide<T>::kN;
   }
-  const int rest = vocab - body * kN;
-  for (int i = thread; i < rest; i += threads) {
-    const int c = i < head ? i : i + body * kN;
-    const float x[1] = {val(row[c])};
-    f(x, c);
+  __device__ __forceinline__ int piece(int i) const { return begin + head + i * Wide<T>::kN; }
+  __device__ __forceinline__ int single(int i) const { return i < head ? begin + i : begin + i + body * Wide<T>::kN; }
+};
+
+// the cluster's first CTA's copy of a shared variable (its own where there is no cluster)
+template <typename V>
+__device__ __forceinline__ V* cluster_first(V* mine) {
+  uint64_t p;
+  asm volatile("mapa.u64 %0, %1, 0;" : "=l"(p) : "l"(mine));
+  return reinterpret_cast<V*>(p);
+}
+
+// Selecting the top_k of a part.
+struct Select {
+  float group[kGroups];
+  uint64_t list[kList];
+  uint64_t best[kMaxCluster * kTop];       // the winners of the cluster's CTAs, in the first one
+  uint64_t warp_key[32];
+  int count, found[kMaxCluster];
+  float bound;
+};
+
+// the top_k-th largest of n floats in shared memory becomes *bound, for n <= blockDim.x
+__device__ __forceinline__ void kth_of(const float* v, int n, int top_k, float* bound) {
+  const int i = (int)threadIdx.x;
+  if (i < n) {
+    const float mine = v[i];
+    int above = 0;
+    for (int j = 0; j < n; j += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(v + j);
+      above += (q.x > mine || (q.x == mine && j < i)) + (q.y > mine || (q.y == mine && j + 1 < i)) + (q.z > mine || (q.z == mine && j + 2 < i)) +
+               (q.w > mine || (q.w == mine && j + 3 < i));
+    }
+    if (above == top_k - 1) *bound = mine;
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ qb_logprobs_args a, int* status) {
-  __shared__ Stats s_stats[kWarps];
-  __shared__ uint64_t s_key[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const T* row = static_cast<const T*>(a.logits) + r / a.inner_rows * a.outer_stride + r % a.inner_rows * a.row_stride;
-    Stats st{neg_inf(), 0.0f, 0.0f};
-    walk_row(row, a.vocab, (int)threadIdx.x, kThreads, [&](const auto& x, int) { add(st, x); });
+template <typename T, int kThreads, bool kEntropy, bool kAlt>
+__global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ qb_logprobs_args a, int parts, int part_len, int* status) {
+  constexpr int kWarps = kThreads / 32, kN = Wide<T>::kN, kAhead = 4;
+  __shared__ Stats s_stats[kWarps], s_parts[kMaxCluster];
+  __shared__ __align__(16) unsigned char s_select[kAlt ? sizeof(Select) : 16];
+  Select& sel = *reinterpret_cast<Select*>(s_select);
+  const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = (int)(blockIdx.x % parts);           // the cluster is `parts` neighbouring CTAs
+  const int64_t r = blockIdx.x / parts;
+  const T* const row = static_cast<const T*>(a.logits) + r / a.inner_rows * a.outer_stride + r % a.inner_rows * a.row_stride;
+  const int from = rank * part_len, to = min(a.vocab, from + part_len);
+  const Part<T> part(row, min(from, a.vocab), max(to, min(from, a.vocab)));
+
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  Stats st{neg_inf(), 0.0f, 0.0f};
+  f2 s2 = 0ull, w2 = 0ull;
+  float bound = neg_inf();
+  const auto list_it = [&](float x, int c) {
+    if (x >= bound && x > neg_inf()) {
+      const int at = atomicAdd(&sel.count, 1);
+      if (at < kList) sel.list[at] = key_of(x, (uint32_t)c);
+    }
+  };
+  const auto look = [&](const Wide<T>& v, float top, int c) {
+    if (top >= bound)
+#pragma unroll
+      for (int k = 0; k < kN; ++k) list_it(val(v.v[k]), c + k);
+  };
+  int i = tid;
+  if (kAlt) {
+    if (tid == 0) sel.count = 0;
+    Wide<T> first;
+    float top = neg_inf();
+    if (i < part.body) {
+      first = load16(row + part.piece(i));
+      top = largest(first);
+      add_piece<kEntropy>(st, s2, w2, first, top);
+    }
+    float over = fmaxf(top, neg_inf());    // a piece of nothing but NaN
+#pragma unroll
+    for (int o = kThreads / kGroups / 2; o > 0; o /= 2) over = fmaxf(over, __shfl_xor_sync(0xffffffffu, over, o));
+    if (tid % (kThreads / kGroups) == 0) sel.group[tid / (kThreads / kGroups)] = over;
+    __syncthreads();
+    kth_of(sel.group, kGroups, a.top_k, &sel.bound);
+    __syncthreads();
+    bound = sel.bound;
+    if (i < part.body) look(first, top, part.piece(i));
+    i += kThreads;
+  }
+  for (; i + (kAhead - 1) * kThreads < part.body; i += kAhead * kThreads) {
+    Wide<T> v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) v[j] = load16(row + part.piece(i + j * kThreads));
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float top = largest(v[j]);
+      add_piece<kEntropy>(st, s2, w2, v[j], top);
+      if (kAlt) look(v[j], top, part.piece(i + j * kThreads));
+    }
+  }
+  for (; i < part.body; i += kThreads) {
+    const Wide<T> v = load16(row + part.piece(i));
+    const float top = largest(v);
+    add_piece<kEntropy>(st, s2, w2, v, top);
+    if (kAlt) look(v, top, part.piece(i));
+  }
+  {
+    float x, y;
+    unpack2(s2, x, y);
+    st.s += x + y;
+    unpack2(w2, x, y);
+    st.w += x + y;
+  }
+  for (int j = tid; j < part.rest; j += kThreads) {
+    const int c = part.single(j);
+    const float x = val(row[c]);
+    add_one<kEntropy>(st, x);
+    if (kAlt) list_it(x, c);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    st = join(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.w, o)});
+  if (lane == 0) s_stats[warp] = st;
+  __syncthreads();
+  if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");    // the first CTA runs: its shared memory may be written
+
+  if (kAlt) {                              // this part's best into sel.best[0 .. found), in no order
+    const int n = sel.count;
+    uint64_t* const out = cluster_first(sel.best) + rank * kTop;
+    int found = min(n, a.top_k);
+    if (n <= kList) {
+      for (int j = tid; j < n; j += kThreads) {
+        const uint64_t mine = sel.list[j];
+        int above = 0;
+        for (int k = 0; k < n; ++k) above += sel.list[k] > mine;
+        if (above < a.top_k) out[above] = mine;
+      }
+    } else {
+      uint64_t below = ~0ull;
+      for (int k = 0; k < a.top_k; ++k) {
+        uint64_t best = 0;
+        const auto see = [&](float x, int c) {
+          const uint64_t key = key_of(x, (uint32_t)c);
+          if (key < below && key > best) best = key;
+        };
+        for (int j = tid; j < part.body; j += kThreads) {
+          const Wide<T> v = load16(row + part.piece(j));
+#pragma unroll
+          for (int e = 0; e < kN; ++e) see(val(v.v[e]), part.piece(j) + e);
+        }
+        for (int j = tid; j < part.rest; j += kThreads) see(val(row[part.single(j)]), part.single(j));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) best = max64(best, (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)best, o));
+        if (lane == 0) sel.warp_key[warp] = best;
+        __syncthreads();
+        for (int j = 0; j < kWarps; ++j) best = max64(best, sel.warp_key[j]);
+        if (tid == 0) out[k] = best;
+        below = best;
+        __syncthreads();
+      }
+      found = a.top_k;                     // more than kList columns: there are as many
+    }
+    if (tid == 0) cluster_first(sel.found)[rank] = found;
+  }
+  if (warp == 0) {
+    st = lane < kWarps ? s_stats[lane] : Stats{neg_inf(), 0.0f, 0.0f};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       st = join(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.w, o)});
-    if (lane == 0) s_stats[warp] = st;
+    if (lane == 0) cluster_first(s_parts)[rank] = st;
+  }
+  if (parts > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank != 0) return;
+  } else {
     __syncthreads();
-    st = s_stats[0];
-    for (int i = 1; i < kWarps; ++i) st = join(st, s_stats[i]);
-    const bool empty = st.m == neg_inf() && st.s == 0.0f;
-    const float logs = logf(st.s);
-    if (threadIdx.x == 0) {
-      const int64_t t = a.targets[r];
-      float lp = 0.0f;
-      if (t != a.ignore_index) {
-        if (t >= 0 && t < a.vocab) {
-          lp = empty ? neg_inf() : (val(row[t]) - st.m) - logs;
-        } else {
-          lp = __int_as_float(0x7fc00000);
-          atomicCAS(status, 0, kStatusTarget);
-        }
+  }
+
+  st = s_parts[0];
+  for (int j = 1; j < parts; ++j) st = join(st, s_parts[j]);
+  const bool empty = st.m == neg_inf() && st.s == 0.0f;
+  const float logs = log2f(st.s);
+  const auto logprob = [&](float x) { return empty ? neg_inf() : fmaf(-logs, kLn2, x - st.m); };
+  if (tid == 0) {
+    const int64_t t = a.targets[r];
+    float lp = 0.0f;
+    if (t != a.ignore_index) {
+      if (t >= 0 && t < a.vocab) {
+        lp = logprob(val(row[t]));
+      } else {
+        lp = quiet_nan();
+        atomicCAS(status, 0, kStatusTarget);
       }
-      a.logprobs[r] = lp;
-      if (a.entropy != nullptr) a.entropy[r] = empty ? 0.0f : logs - st.w / st.s;
-      if (a.lse != nullptr) a.lse[r] = empty ? neg_inf() : st.m + logs;
     }
-    uint64_t below = ~0ull;
-    for (int k = 0; k < a.top_k; ++k) {
-      uint64_t best = 0;
-      walk_row(row, a.vocab, (int)threadIdx.x, kThreads, [&](const auto& x, int c) {
-#pragma unroll
-        for (int j = 0; j < (int)(sizeof(x) / sizeof(float)); ++j) {
-          const uint64_t key = key_of(x[j], (uint32_t)(c + j));
-          if (key < below && key > best) best = key;
-        }
-      });
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)best, o));
-      if (lane == 0) s_key[warp] = best;
-      __syncthreads();
-      for (int i = 0; i < kWarps; ++i) best = max(best, s_key[i]);
-      if (threadIdx.x == 0) {
-        a.top_ids[r * a.top_k + k] = column_of(best);
-        a.top_logprobs[r * a.top_k + k] = empty ? neg_inf() : (value_of(best) - st.m) - logs;
+    a.logprobs[r] = lp;
+    if (kEntropy) a.entropy[r] = empty ? 0.0f : (logs - st.w / st.s) * kLn2;
+    if (a.lse != nullptr) a.lse[r] = empty ? neg_inf() : fmaf(logs, kLn2, st.m);
+  }
+  if (kAlt) {
+    int n = 0;
+    for (int j = 0; j < parts; ++j) n += sel.found[j];
+    for (int j = tid; j < parts * kTop; j += kThreads) {
+      if (j % kTop >= sel.found[j / kTop]) continue;
+      const uint64_t mine = sel.best[j];
+      int above = 0;
+      for (int q = 0; q < parts; ++q)
+        for (int k = 0; k < sel.found[q]; ++k) above += sel.best[q * kTop + k] > mine;
+      if (above < a.top_k) {
+        a.top_ids[r * a.top_k + above] = column_of(mine);
+        a.top_logprobs[r * a.top_k + above] = logprob(value_of(mine));
       }
-      below = best;
-      __syncthreads();
     }
-    __syncthreads();
+    // fewer numbers above -inf than asked for: the lowest of the other columns (-inf, or NaN in a row without a distribution)
+    if (tid == 0)
+      for (int c = 0; n < a.top_k; ++c) {
+        const float x = val(row[c]);
+        if (x > neg_inf()) continue;
+        a.top_ids[r * a.top_k + n] = c;
+        a.top_logprobs[r * a.top_k + n] = logprob(x);
+        ++n;
+      }
   }
 }
 
@@ -217,6 +410,28 @@ int check_logprobs(const qb_logprobs_args* a, const char* who) {
   return QB_OK;
 }
 
+template <typename T, int kThreads, bool kEntropy, bool kAlt>
+int launch_logprobs(const qb_logprobs_args& a, int* status, cudaStream_t st) {
+  // CTAs of a row: enough of them to give every multiprocessor two, with a piece per thread at least
+  int64_t parts = 1;
+  while (parts < kMaxCluster && a.rows * parts * 2 <= (int64_t)sm_count() * 2 && a.vocab / (parts * 2) >= kThreads * Wide<T>::kN) parts *= 2;
+  const int64_t unit = 128 / (int64_t)sizeof(T), part_len = ceil_div(ceil_div(a.vocab, parts), unit) * unit;
+  QB_REQUIRE(a.rows * parts < (1ll << 31), QB_ERR_TOO_LARGE, "logprobs_fwd: too many rows");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&cfg, logprobs_kernel<T, kThreads, kEntropy, kAlt>, a, (int)parts, (int)part_len, status);
+  QB_LAUNCH_OK("logprobs_kernel");
+  return QB_OK;
+}
+
 template <typename F>
 int by_type(int dtype, F f) {
   return dtype == 0 ? f(float{}) : dtype == 1 ? f(__half{}) : f(__nv_bfloat16{});
@@ -238,9 +453,9 @@ extern "C" int qb_logprobs_fwd(const qb_logprobs_args* a, void* stream) {
   QB_REQUIRE(status != nullptr, QB_ERR_CUDA, "device status word unavailable");
   return by_type(a->dtype, [&](auto t) -> int {
     using T = decltype(t);
-    logprobs_kernel<T><<<(unsigned)std::min<int64_t>(a->rows, 1 << 20), kThreads, 0, (cudaStream_t)stream>>>(*a, status);
-    QB_LAUNCH_OK("logprobs_kernel");
-    return QB_OK;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a->top_k > 0) return a->entropy ? launch_logprobs<T, 512, true, true>(*a, status, st) : launch_logprobs<T, 512, false, true>(*a, status, st);
+    return a->entropy ? launch_logprobs<T, 256, true, false>(*a, status, st) : launch_logprobs<T, 256, false, false>(*a, status, st);
   });
 }
 

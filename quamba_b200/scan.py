@@ -55,7 +55,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
 
     Differentiable once, in every floating-point argument, the initial and the final state included.  States, sums over
     channels and parameters' gradients are float32, summed in a fixed order.  For the backward pass the state is kept every
-    16 tokens (a quarter of dstate bytes per token and channel).  To capture forward and backward into a CUDA graph let no
+    8 tokens (half of dstate, rounded up to 16, 32 or 64, bytes per token and channel).  To capture forward and backward into a CUDA graph let no
     eager graph of the same leaves be alive, as for every torch operator."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, D, z, dt_bias, initial_state)):
         y, last = _SelectiveScan.apply(x, dt, A, B, C, D, z, dt_bias, bool(dt_softplus), initial_state, lengths)

@@ -64,8 +64,8 @@ def test_workspace_sizes():
     lib = _lib.lib()
     for f in (lib.qb_float_scan_workspace_bytes, lib.qb_float_scan_checkpoint_bytes):
         f.restype = ctypes.c_int64
-    assert lib.qb_float_scan_checkpoint_bytes(1, 16, 32, 1, 16) == 512 * 4
-    assert lib.qb_float_scan_checkpoint_bytes(2, 17, 33, 1, 16) == 2 * 2 * 2 * 512 * 4
+    assert lib.qb_float_scan_checkpoint_bytes(1, 16, 32, 1, 16) == 2 * 32 * 16 * 4
+    assert lib.qb_float_scan_checkpoint_bytes(2, 17, 33, 1, 20) == 2 * 3 * 33 * 32 * 4
     assert lib.qb_float_scan_checkpoint_bytes(1, 16, 32, 5, 16) == -1
     assert lib.qb_float_scan_workspace_bytes(1, 16, 32, 1, 65, 1) == -1
     assert lib.qb_float_scan_workspace_bytes(4, 2048, 5120, 1, 16, 1) > lib.qb_float_scan_workspace_bytes(4, 2048, 5120, 1, 16, 0) >= 0
