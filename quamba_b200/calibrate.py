@@ -18,6 +18,8 @@ from .mixer import W4A8QMamba2, W8A8QMamba2
 from .model import QuambaConfig, QuambaLMHeadModel
 from .modules import W4A8B16O16Linear, W8A8B16O16Linear
 from .norm import QRMSNorm
+from .scan import selective_scan
+from .scoring import next_token_targets, token_logprobs
 
 __all__ = ["Mamba1Float", "Mamba1LMFloat", "Mamba2Float", "Mamba2LMFloat", "calibrate", "calibrate_mamba1", "quantize_model",
            "quantize_mamba1_model", "ssd_float"]
@@ -239,11 +241,13 @@ def quantize_model(model: Mamba2LMFloat, act_scales, w_bits=4, quantize_embeddin
 class Mamba1Float(nn.Module):
     """Float Mamba1 mixer (the role of the reference's ``MambaSimple``) with its tap points: in_proj -> x | z -> causal
     conv1d + SiLU -> x_proj -> dt | B | C -> dt_proj (bias kept apart in ``dt_proj_bias``) -> selective scan with gate z ->
-    Hadamard rotation -> out_proj.  ``taps`` (dict name -> running absmax) is filled when given."""
+    Hadamard rotation -> out_proj.  ``taps`` (dict name -> running absmax) is filled when given.  ``scan_kernel`` runs the scan on
+    :func:`quamba_b200.selective_scan` (CUDA, gradients included) instead of token by token in torch."""
 
     def __init__(self, d_model, d_state=16, d_conv=4, expand=2, dt_rank="auto", layer_idx=None, w4_group_size=None,
-                 generator=None, device=None):
+                 generator=None, device=None, scan_kernel=False):
         super().__init__()
+        self.scan_kernel = scan_kernel
         self.d_model, self.d_state, self.d_conv, self.expand, self.layer_idx = d_model, d_state, d_conv, expand, layer_idx
         self.d_inner = expand * d_model
         self.dt_rank = math.ceil(d_model / 16) if dt_rank == "auto" else dt_rank
@@ -281,6 +285,14 @@ class Mamba1Float(nn.Module):
         x = tap("x_proj:input", F.silu(self.conv1d(x)[..., :l]))
         x_dbl = tap("x_proj:output", self.x_proj(x.transpose(1, 2)))           # (b, l, R + 2N)
         dt = tap("dt_proj:output", self.dt_proj(x_dbl[..., :R])).transpose(1, 2)   # (b, D, l), bias not added yet
+        if self.scan_kernel:
+            y, h = selective_scan(x.transpose(1, 2).contiguous(), dt.transpose(1, 2), -torch.exp(self.A_log.float()), x_dbl[..., R:R + N],
+                                  x_dbl[..., R + N:], D=self.D.float(), z=z.transpose(1, 2), dt_bias=self.dt_proj_bias.float(), dt_softplus=True,
+                                  return_final_state=True)
+            tap("ssm_state_act:input", h)
+            if state is not None:
+                state["ssm"] = h
+            return self.out_proj(tap("out_proj:input", hadamard_transform(y.float())).to(u.dtype))
         Bm, Cm = x_dbl[..., R:R + N].float(), x_dbl[..., R + N:].float()      # (b, l, N)
         delta = F.softplus(dt.float() + self.dt_proj_bias.float()[None, :, None])
         A = -torch.exp(self.A_log.float())
@@ -314,7 +326,7 @@ class Mamba1LMFloat(nn.Module):
     Mamba1 counterpart of :class:`Mamba2LMFloat` (same tap convention: one dict per layer plus one for the head)."""
 
     def __init__(self, d_model=2560, n_layer=64, vocab_size=50288, d_state=16, d_conv=4, expand=2, w4_group_size=None, seed=0,
-                 device=None):
+                 device=None, scan_kernel=False):
         super().__init__()
         g = torch.Generator(device=device).manual_seed(seed)
         self.d_model, self.n_layer, self.vocab_size = d_model, n_layer, vocab_size
@@ -327,12 +339,11 @@ class Mamba1LMFloat(nn.Module):
         if w4_group_size is not None:
             self.lm_head.w4_group_size = w4_group_size
         self.mixers = nn.ModuleList([Mamba1Float(d_model, layer_idx=i, w4_group_size=w4_group_size, generator=g, device=device,
-                                                 **self.ssm_cfg) for i in range(n_layer)])
+                                                 scan_kernel=scan_kernel, **self.ssm_cfg) for i in range(n_layer)])
         self.norms = nn.ModuleList([RMSNormFloat(d_model).to(device) for _ in range(n_layer)])
         self.norm_f = RMSNormFloat(d_model).to(device)
 
-    @torch.no_grad()
-    def forward(self, input_ids, taps=None):
+    def _logits(self, input_ids, taps=None):
         h = self.embedding(input_ids)
         residual = torch.zeros_like(h, dtype=torch.float32)
         for i, (norm, mixer) in enumerate(zip(self.norms, self.mixers)):
@@ -343,6 +354,16 @@ class Mamba1LMFloat(nn.Module):
         if taps is not None:
             Mamba2Float._tap(taps[-1], "lm_head:input", y)
         return self.lm_head(y.to(h.dtype))
+
+    @torch.no_grad()
+    def forward(self, input_ids, taps=None):
+        return self._logits(input_ids, taps)
+
+    def token_logprobs(self, input_ids, lengths=None, top_k=0, return_entropy=False):
+        """:class:`quamba_b200.TokenLogprobs` (batch, seqlen - 1) of every token after the first given those before it, differentiable
+        in the parameters: ``-model.token_logprobs(ids).logprobs.mean()`` is the loss of a fine-tuning step.  ``lengths``
+        (batch,): tokens from there on count 0.  CUDA only; build the model with ``scan_kernel=True``."""
+        return token_logprobs(self._logits(input_ids)[:, :-1], next_token_targets(input_ids, lengths), top_k=top_k, return_entropy=return_entropy)
 
 
 @torch.no_grad()

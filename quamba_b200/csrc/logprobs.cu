@@ -7,10 +7,10 @@
 // leaves at the memory's speed.  Many rows take a CTA each; few rows a cluster of up to eight, whose parts are joined over
 // distributed shared memory.
 //
-// Alternatives in the same pass.  Of the first piece of every thread the maxima of 128 groups are ranked: the top_k-th of them is a bound
-// that at least top_k values reach, so what is below it never counts again.  Values that reach it are listed (some hundreds), and
-// the list is ranked at the end by (value, column).  A list that runs over (long plateaus of equal values, rows that rise to
-// the end) sends the row's part to top_k searches for the largest key below the last.
+// Alternatives in the same pass.  The maxima of 128 groups of a CTA's threads over their first four pieces are ranked: the top_k-th of
+// them is a bound that at least top_k values reach, so what is below it never counts again.  Values that reach it are listed
+// (some tens), and the list is ranked at the end by (value, column).  A list that runs over (long plateaus of equal
+// values, rows that rise to the end) sends the row's part to top_k searches for the largest key below the last.
 //
 // Bound by the row's bytes: read once forward; read and written once backward.
 #include <algorithm>
@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kStatusTarget = 502;       // keep in step with qb_read_device_status (lib.cu)
 constexpr int kMaxCluster = 8;
-constexpr int kGroups = 128;             // groups of threads whose first maxima are ranked
+constexpr int kMaxGroups = 128;          // groups of threads whose first maxima are ranked
 constexpr int kList = 2048;              // candidates listed per CTA
 constexpr int kTop = QB_LOGPROBS_MAX_TOP;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -41,6 +41,10 @@ template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ void narrow2(float* p, float x, float y) { p[0] = x; p[1] = y; }
+__device__ __forceinline__ void narrow2(__half* p, float x, float y) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y); }
+__device__ __forceinline__ void narrow2(__nv_bfloat16* p, float x, float y) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y); }
 
 template <typename T>
 __device__ __forceinline__ Wide<T> load16(const T* p) {
@@ -147,7 +151,7 @@ __device__ __forceinline__ V* cluster_first(V* mine) {
 
 // Selecting the top_k of a part.
 struct Select {
-  float group[kGroups];
+  float group[kMaxGroups];
   uint64_t list[kList];
   uint64_t best[kMaxCluster * kTop];       // the winners of the cluster's CTAs, in the first one
   uint64_t warp_key[32];
@@ -157,22 +161,20 @@ struct Select {
 
 // the top_k-th largest of n floats in shared memory becomes *bound, for n <= blockDim.x
 __device__ __forceinline__ void kth_of(const float* v, int n, int top_k, float* bound) {
-  const int i = (int)threadIdx.x;
-  if (i < n) {
-    const float mine = v[i];
-    int above = 0;
-    for (int j = 0; j < n; j += 4) {
-      const float4 q = *reinterpret_cast<const float4*>(v + j);
-      above += (q.x > mine || (q.x == mine && j < i)) + (q.y > mine || (q.y == mine && j + 1 < i)) + (q.z > mine || (q.z == mine && j + 2 < i)) +
-               (q.w > mine || (q.w == mine && j + 3 < i));
-    }
-    if (above == top_k - 1) *bound = mine;
+  if ((int)threadIdx.x >= n) return;
+  const float mine = v[threadIdx.x];
+  int above = 0, reach = 0;
+  for (int j = 0; j < n; j += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(v + j);
+    above += (q.x > mine) + (q.y > mine) + (q.z > mine) + (q.w > mine);
+    reach += (q.x >= mine) + (q.y >= mine) + (q.z >= mine) + (q.w >= mine);
   }
+  if (above < top_k && reach >= top_k) *bound = mine;      // equal values pass together and write the same
 }
 
 template <typename T, int kThreads, bool kEntropy, bool kAlt>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ qb_logprobs_args a, int parts, int part_len, int* status) {
-  constexpr int kWarps = kThreads / 32, kN = Wide<T>::kN, kAhead = 4;
+__global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) logprobs_kernel(const __grid_constant__ qb_logprobs_args a, int parts, int part_len, int* status) {
+  constexpr int kWarps = kThreads / 32, kN = Wide<T>::kN, kAhead = 4, kGroups = kThreads < kMaxGroups ? kThreads : kMaxGroups;
   __shared__ Stats s_stats[kWarps], s_parts[kMaxCluster];
   __shared__ __align__(16) unsigned char s_select[kAlt ? sizeof(Select) : 16];
   Select& sel = *reinterpret_cast<Select*>(s_select);
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
   const int from = rank * part_len, to = min(a.vocab, from + part_len);
   const Part<T> part(row, min(from, a.vocab), max(to, min(from, a.vocab)));
 
-  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   Stats st{neg_inf(), 0.0f, 0.0f};
   f2 s2 = 0ull, w2 = 0ull;
   float bound = neg_inf();
@@ -201,14 +203,8 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
   int i = tid;
   if (kAlt) {
     if (tid == 0) sel.count = 0;
-    Wide<T> first;
-    float top = neg_inf();
-    if (i < part.body) {
-      first = load16(row + part.piece(i));
-      top = largest(first);
-      add_piece<kEntropy>(st, s2, w2, first, top);
-    }
-    float over = fmaxf(top, neg_inf());    // a piece of nothing but NaN
+    float over = neg_inf();                // a piece of nothing but NaN counts as -inf
+    for (int j = tid; j < min(part.body, kAhead * kThreads); j += kThreads) over = fmaxf(over, largest(load16(row + part.piece(j))));
 #pragma unroll
     for (int o = kThreads / kGroups / 2; o > 0; o /= 2) over = fmaxf(over, __shfl_xor_sync(0xffffffffu, over, o));
     if (tid % (kThreads / kGroups) == 0) sel.group[tid / (kThreads / kGroups)] = over;
@@ -216,8 +212,6 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
     kth_of(sel.group, kGroups, a.top_k, &sel.bound);
     __syncthreads();
     bound = sel.bound;
-    if (i < part.body) look(first, top, part.piece(i));
-    i += kThreads;
   }
   for (; i + (kAhead - 1) * kThreads < part.body; i += kAhead * kThreads) {
     Wide<T> v[kAhead];
@@ -254,7 +248,9 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
     st = join(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.w, o)});
   if (lane == 0) s_stats[warp] = st;
   __syncthreads();
-  if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");    // the first CTA runs: its shared memory may be written
+  // The first CTA runs: its shared memory may be written.  (None of the cluster barriers is the .aligned form: that one wants whole
+  // warps at a time, and lanes leave the loops over listed keys below one by one.)
+  if (parts > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 
   if (kAlt) {                              // this part's best into sel.best[0 .. found), in no order
     const int n = sel.count;
@@ -302,7 +298,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
     if (lane == 0) cluster_first(s_parts)[rank] = st;
   }
   if (parts > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     if (rank != 0) return;
   } else {
     __syncthreads();
@@ -344,7 +340,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
     }
     // fewer numbers above -inf than asked for: the lowest of the other columns (-inf, or NaN in a row without a distribution)
     if (tid == 0)
-      for (int c = 0; n < a.top_k; ++c) {
+      for (int c = 0; c < a.vocab && n < a.top_k; ++c) {
         const float x = val(row[c]);
         if (x > neg_inf()) continue;
         a.top_ids[r * a.top_k + n] = c;
@@ -354,10 +350,10 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
   }
 }
 
-// d_logits = g ([i == target] - p_i) - h p_i (log p_i + H); pieces of a row, kPieces vectors per thread
+// d_logits = g ([i == target] - p_i) - h p_i (log p_i + H); pieces of a row, kPieces per thread
 constexpr int kBwdThreads = 256, kPieces = 4;
-template <typename T>
-__global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const __grid_constant__ qb_logprobs_args a, int parts) {
+template <typename T, bool kEntropy>
+__global__ void __launch_bounds__(kBwdThreads, 6) logprobs_bwd_kernel(const __grid_constant__ qb_logprobs_args a, int parts) {
   constexpr int kN = Wide<T>::kN;
   const int64_t r = blockIdx.x / parts;
   const int part = (int)(blockIdx.x % parts);
@@ -365,39 +361,55 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const __grid_
   T* out = static_cast<T*>(a.d_logits) + r / a.inner_rows * a.d_outer_stride + r % a.inner_rows * a.d_row_stride;
   const int64_t t = a.targets[r];
   const bool kept = t != a.ignore_index && t >= 0 && t < a.vocab;
+  const int target = kept ? (int)t : -1;
   const float g = kept && a.d_logprobs != nullptr ? a.d_logprobs[r] : 0.0f;
-  const float h = a.d_entropy != nullptr ? a.d_entropy[r] : 0.0f, H = a.d_entropy != nullptr ? a.entropy[r] : 0.0f;
+  const float h = kEntropy ? a.d_entropy[r] : 0.0f, H = kEntropy ? a.entropy[r] : 0.0f;
   const float lse = a.lse[r];
   const bool empty = lse == neg_inf();
   const float base = fmaf(h, H, g);                    // d = -p (g + h (log p + H))
-  auto one = [&](float x, int c) {
-    const float lp = x - lse, p = fast_exp2(lp * kLog2e);
-    float d = -p * fmaf(h, fmaxf(lp, kFar), base);
-    if (c == t && kept) d += g;
-    return empty ? 0.0f : d;
+  const f2 mm = pack2(-lse, -lse), l2 = pack2(kLog2e, kLog2e), hh = pack2(-h, -h), bb = pack2(-base, -base);
+  auto two = [&](float x, float y) {
+    const f2 lp = add2(pack2(x, y), mm);
+    float u, v;
+    unpack2(mul2(lp, l2), u, v);
+    const f2 p = pack2(fast_exp2(u), fast_exp2(v));
+    if (!kEntropy) return mul2(p, bb);
+    unpack2(lp, u, v);
+    return mul2(p, fma2(hh, pack2(fmaxf(u, kFar), fmaxf(v, kFar)), bb));
   };
   const uintptr_t ai = reinterpret_cast<uintptr_t>(row) & 15, ao = reinterpret_cast<uintptr_t>(out) & 15;
   const int head = ai == ao ? min(a.vocab, (int)((16 - ai) & 15) / (int)sizeof(T)) : a.vocab;   // not alike: one by one
   const int body = (a.vocab - head) / kN;
   constexpr int kStep = kBwdThreads * kPieces;
   for (int i0 = part * kStep; i0 < body; i0 += parts * kStep) {
+    Wide<T> v[kPieces];
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
       const int i = i0 + k * kBwdThreads + (int)threadIdx.x;
-      if (i < body) {
-        const int c = head + i * kN;
-        const Wide<T> v = load16(row + c);
-        Wide<T> o;
+      if (i < body) v[k] = load16(row + head + i * kN);
+    }
 #pragma unroll
-        for (int j = 0; j < kN; ++j) o.v[j] = narrow<T>(one(val(v.v[j]), c + j));
-        *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(o.v);
-      }
+    for (int k = 0; k < kPieces; ++k) {
+      const int i = i0 + k * kBwdThreads + (int)threadIdx.x, c = head + i * kN;
+      if (i >= body) break;
+      float d[kN];
+#pragma unroll
+      for (int j = 0; j < kN; j += 2) unpack2(two(val(v[k].v[j]), val(v[k].v[j + 1])), d[j], d[j + 1]);
+      if (empty || (unsigned)(target - c) < (unsigned)kN)
+#pragma unroll
+        for (int j = 0; j < kN; ++j) d[j] = empty ? 0.0f : d[j] + (c + j == target ? g : 0.0f);
+      Wide<T> o;
+#pragma unroll
+      for (int j = 0; j < kN; j += 2) narrow2(o.v + j, d[j], d[j + 1]);
+      *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(o.v);
     }
   }
   const int rest = a.vocab - body * kN;
   for (int i = part * kBwdThreads + (int)threadIdx.x; i < rest; i += parts * kBwdThreads) {
     const int c = i < head ? i : i + body * kN;
-    out[c] = narrow<T>(one(val(row[c]), c));
+    float d, twin;
+    unpack2(two(val(row[c]), 0.0f), d, twin);
+    out[c] = narrow<T>(empty ? 0.0f : d + (c == target ? g : 0.0f));
   }
 }
 
@@ -412,9 +424,10 @@ int check_logprobs(const qb_logprobs_args* a, const char* who) {
 
 template <typename T, int kThreads, bool kEntropy, bool kAlt>
 int launch_logprobs(const qb_logprobs_args& a, int* status, cudaStream_t st) {
-  // CTAs of a row: enough of them to give every multiprocessor two, with a piece per thread at least
+  // CTAs of a row: as many in all as are resident at once, with a piece per thread at least
+  constexpr int kResident = kAlt && kThreads == 512 ? 2 : 2048 / kThreads;
   int64_t parts = 1;
-  while (parts < kMaxCluster && a.rows * parts * 2 <= (int64_t)sm_count() * 2 && a.vocab / (parts * 2) >= kThreads * Wide<T>::kN) parts *= 2;
+  while (parts < kMaxCluster && a.rows * parts * 2 <= (int64_t)sm_count() * kResident && a.vocab / (parts * 2) >= kThreads * Wide<T>::kN) parts *= 2;
   const int64_t unit = 128 / (int64_t)sizeof(T), part_len = ceil_div(ceil_div(a.vocab, parts), unit) * unit;
   QB_REQUIRE(a.rows * parts < (1ll << 31), QB_ERR_TOO_LARGE, "logprobs_fwd: too many rows");
   cudaLaunchConfig_t cfg = {};
@@ -426,10 +439,16 @@ int launch_logprobs(const qb_logprobs_args& a, int* status, cudaStream_t st) {
   attr[0].val.clusterDim.x = (unsigned)parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
   (void)cudaLaunchKernelEx(&cfg, logprobs_kernel<T, kThreads, kEntropy, kAlt>, a, (int)parts, (int)part_len, status);
   QB_LAUNCH_OK("logprobs_kernel");
   return QB_OK;
+}
+
+template <typename T, int kThreads, int kAltThreads>
+int launch_for(const qb_logprobs_args& a, int* status, cudaStream_t st) {
+  if (a.top_k > 0) return a.entropy ? launch_logprobs<T, kAltThreads, true, true>(a, status, st) : launch_logprobs<T, kAltThreads, false, true>(a, status, st);
+  return a.entropy ? launch_logprobs<T, kThreads, true, false>(a, status, st) : launch_logprobs<T, kThreads, false, false>(a, status, st);
 }
 
 template <typename F>
@@ -454,8 +473,8 @@ extern "C" int qb_logprobs_fwd(const qb_logprobs_args* a, void* stream) {
   return by_type(a->dtype, [&](auto t) -> int {
     using T = decltype(t);
     cudaStream_t st = (cudaStream_t)stream;
-    if (a->top_k > 0) return a->entropy ? launch_logprobs<T, 512, true, true>(*a, status, st) : launch_logprobs<T, 512, false, true>(*a, status, st);
-    return a->entropy ? launch_logprobs<T, 256, true, false>(*a, status, st) : launch_logprobs<T, 256, false, false>(*a, status, st);
+    // short rows take two warps: a CTA's set-up and reduction then weigh less
+    return (int64_t)a->vocab * (int64_t)sizeof(T) < 16384 ? launch_for<T, 64, 64>(*a, status, st) : launch_for<T, 256, 512>(*a, status, st);
   });
 }
 
@@ -470,7 +489,8 @@ extern "C" int qb_logprobs_bwd(const qb_logprobs_args* a, void* stream) {
   QB_REQUIRE(a->rows * parts < (1ll << 31), QB_ERR_TOO_LARGE, "logprobs_bwd: too many rows");
   return by_type(a->dtype, [&](auto t) -> int {
     using T = decltype(t);
-    logprobs_bwd_kernel<T><<<(unsigned)(a->rows * parts), kBwdThreads, 0, (cudaStream_t)stream>>>(*a, (int)parts);
+    if (a->d_entropy != nullptr) logprobs_bwd_kernel<T, true><<<(unsigned)(a->rows * parts), kBwdThreads, 0, (cudaStream_t)stream>>>(*a, (int)parts);
+    else logprobs_bwd_kernel<T, false><<<(unsigned)(a->rows * parts), kBwdThreads, 0, (cudaStream_t)stream>>>(*a, (int)parts);
     QB_LAUNCH_OK("logprobs_bwd_kernel");
     return QB_OK;
   });

@@ -23,6 +23,7 @@ from . import modules as _modules
 from . import _lib
 from . import ops
 from .norm import QRMSNorm
+from .scoring import TokenLogprobs, next_token_targets, token_logprobs
 
 __all__ = ["QuambaConfig", "InferenceParams", "Block", "QuambaMixerModel", "QuambaLMHeadModel", "GraphRunner"]
 
@@ -254,6 +255,26 @@ class QuambaLMHeadModel(nn.Module):
             return CausalLMOutput(logits=bb.decode_step_fused(input_ids, inference_params, self.lm_head)[:, None])
         hidden_states = bb(input_ids, inference_params=inference_params, num_last_tokens=num_last_tokens, **mixer_kwargs)
         return CausalLMOutput(logits=self.lm_head(hidden_states))
+
+    @torch.no_grad()
+    def score(self, input_ids, lengths=None, top_k=0, return_entropy=False, rows_per_chunk=4096):
+        """How likely each token after the first is given those before it: :class:`quamba_b200.TokenLogprobs` with (batch, seqlen - 1)
+        ``logprobs`` (``exp(-logprobs.mean())`` is the text's perplexity), ``entropy`` and the ``top_k`` alternatives at every
+        position.  ``lengths`` (batch,): tokens from there on are padding and count 0.  The head runs on ``rows_per_chunk`` positions at a
+        time, so that no more logits than those exist; its columns past ``config.vocab_size`` are left out."""
+        batch, seqlen = input_ids.shape
+        rows = batch * max(0, seqlen - 1)
+        targets = next_token_targets(input_ids, lengths).reshape(rows)
+        hidden = self.backbone(input_ids)[:, :-1].flatten(0, 1) if rows else None
+        parts = []
+        for i in range(0, max(rows, 1), rows_per_chunk):
+            logits = (self.lm_head(hidden[i:i + rows_per_chunk])[:, :self.config.vocab_size] if rows
+                      else torch.empty((0, self.config.vocab_size), dtype=torch.float16, device=input_ids.device))
+            parts.append(token_logprobs(logits, targets[i:i + rows_per_chunk], top_k=top_k, return_entropy=return_entropy))
+        joined = [None if p[0] is None else torch.cat(p) for p in zip(*parts)]
+        from . import check_device_status
+        check_device_status()
+        return TokenLogprobs(*(None if t is None else t.view(batch, max(0, seqlen - 1), *t.shape[1:]) for t in joined))
 
     # ---- CUDA-graph runners ------------------------------------------------------------------------------------------
     def capture_prefill(self, batch_size, seqlen, stream=None):

@@ -64,7 +64,6 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     return (y, last) if return_final_state else y
 
 
-@torch.no_grad()
 def selective_scan_update(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, state_out=None):
     """One token per sequence: x, dt, z (batch, dim), B, C (batch, dstate) or (batch, groups, dstate), state float32
     (batch, dim, dstate), contiguous in its last dim.  Returns y (batch, dim); the state is advanced in place, or written to

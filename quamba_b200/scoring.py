@@ -6,7 +6,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-__all__ = ["TokenLogprobs", "token_logprobs"]
+__all__ = ["TokenLogprobs", "next_token_targets", "token_logprobs"]
 
 _n = _lib.native
 
@@ -51,3 +51,13 @@ def token_logprobs(logits, targets, top_k=0, return_entropy=False, ignore_index=
     else:
         lp, ent, _, top, ids = _n().logprobs_fwd(logits, targets, top_k, return_entropy, ignore_index)
     return TokenLogprobs(lp, ent, top, ids)
+
+
+def next_token_targets(input_ids, lengths=None, ignore_index=-100):
+    """The targets (batch, seqlen - 1) of a batch of token ids: each position's next token, ``ignore_index`` where that is at or past
+    ``lengths[b]``."""
+    targets = input_ids[:, 1:]
+    if lengths is None:
+        return targets
+    lengths = torch.as_tensor(lengths, device=input_ids.device)
+    return targets.masked_fill(torch.arange(1, input_ids.shape[1], device=input_ids.device)[None] >= lengths[:, None], ignore_index)
