@@ -10,6 +10,7 @@
 // Bound: dstate exponentials per (token, channel) on the MUFU pipe (16 results per clock and SM): 16 states cost 1 clock per
 // (token, channel) and SM, while its bytes (8 at 16 bits) take 0.18 clocks of HBM time.
 #include <algorithm>
+#include <cstddef>
 #include "tc_common.cuh"
 
 namespace qb {
@@ -54,30 +55,24 @@ __device__ __forceinline__ void softplus_series(float& a, float& b) {
   p = fma2(w, p, splat(1.0f));
   unpack2(fma2(add2(s, s), p, pack2(fmaxf(a, 0.0f), fmaxf(b, 0.0f))), a, b);
 }
-__device__ __forceinline__ float sigmoid_fast(float v) {
-  const float e = fast_exp2(-fabsf(v) * kLog2e), r = rcp_fast(1.0f + e);
-  return v >= 0.0f ? r : e * r;
-}
+__device__ __forceinline__ float sigmoid_fast(float v) { return rcp_fast(1.0f + fast_exp2(v * -kLog2e)); }
 __device__ __forceinline__ f2 exp2_pair(f2 x) {
   float a, b;
   unpack2(x, a, b);
   return pack2(fast_exp2(a), fast_exp2(b));
 }
 
-// 2^x to within rounding: the nearest integer by the adder, the fraction's power by its series (|f| <= 1/2, the term left out is
-// below 2^-27).  Results below 2^-126 are zero, above 2^127 infinite.
-__device__ __forceinline__ float exp2_series(float x) {
-  const float c = fminf(fmaxf(x, -127.0f), 128.0f);
-  const float i = rintf(c), f = (c - i) * kLn2;
-  float p = fmaf(f, 1.0f / 5040, 1.0f / 720);
-  p = fmaf(f, p, 1.0f / 120);
-  p = fmaf(f, p, 1.0f / 24);
-  p = fmaf(f, p, 1.0f / 6);
-  p = fmaf(f, p, 0.5f);
-  p = fmaf(f, p, 1.0f);
-  p = fmaf(f, p, 1.0f);
-  const float r = p * __int_as_float(((int)i + 127) << 23);       // exponent 0: zero, 255: infinite
-  return x != x ? x : r;
+// 2^x for two values with no systematic error where it would last: near zero, where a state lives long, by its series (|x| < 1/16: the
+// term left out is below 2^-29), elsewhere from the exponential unit.
+__device__ __forceinline__ f2 exp2_fine(f2 x) {
+  f2 p = fma2(x, splat(9.6181291e-3f), splat(5.5504109e-2f));
+  p = fma2(x, p, splat(0.24022651f));
+  p = fma2(x, p, splat(kLn2));
+  p = fma2(x, p, splat(1.0f));
+  float a, b, u, v;
+  unpack2(x, a, b);
+  unpack2(p, u, v);
+  return pack2(fabsf(a) < 0.0625f ? u : fast_exp2(a + kLift), fabsf(b) < 0.0625f ? v : fast_exp2(b + kLift));
 }
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -175,25 +170,69 @@ __device__ __forceinline__ float own_channel(const float (&v)[kCh], int q) {
   return a;
 }
 
-// v summed over the lanes of one q, which halve the list between them until it has one value; the sums go to out
-template <int kCount, int kQ>
-__device__ __forceinline__ void over_groups(float (&v)[kCount], int lane, float* out) {
-  int at = 0, left = kCount;
+// Sums over the lanes of one q of kNp values each, four tokens at a time.  Sixteen values a lane go through shared memory: a lane leaves
+// them as 16-byte pieces, then every lane adds up an output piece (t, n .. n + 3) over the groups (2 x 1024 tokens of 5120 channels of 64
+// states: 1.76 ms, 2.44 by shuffles).  Eight go by shuffles that halve the list at every step: there the way through
+// shared memory takes fewer instructions but more time (1.15 ms for 8 x 1024 tokens of 5120 channels of 16 states, 1.10 by shuffles).
+template <typename G, bool kShared = G::kNp == 16>
+struct GroupSums {
+  static constexpr int kTokens = 4, kRow = 32 * G::kNp + 16, kPer = G::kNp / 4;
+  float v[kTokens][kRow];
+  static __device__ __forceinline__ int place(int lane, int piece) { return lane * G::kNp + (piece ^ (kPer == 2 ? (lane >> 2) & 1 : (lane >> 1) & 3)) * 4; }
+  __device__ __forceinline__ void put(int t, int lane, const f2 (&s)[G::kPairs], float*) {
 #pragma unroll
-  for (int bit = 16; bit >= kQ; bit >>= 1) {
-    const bool up = lane & bit;
-    if (left > 1) {
-      left /= 2;
-#pragma unroll
-      for (int k = 0; k < left; ++k) v[k] = (up ? v[left + k] : v[k]) + __shfl_xor_sync(0xffffffffu, up ? v[k] : v[left + k], bit);
-      at += up ? left : 0;
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);     // both hold the sum
-    }
+    for (int p = 0; p < kPer; ++p) *reinterpret_cast<ulonglong2*>(&v[t][place(lane, p)]) = make_ulonglong2(s[2 * p], s[2 * p + 1]);
   }
+  // out: [4][out_row] with the kN sums of a token first
+  __device__ __forceinline__ void take(int lane, float* out, int out_row) const {
+    __syncwarp();
+    constexpr int kPieces = kTokens * G::kN / 4, kShare = kPieces < 32 ? 32 / kPieces : 1, kGroups = 32 / G::kQ / kShare;
 #pragma unroll
-  for (int k = 0; k < left; ++k) out[at + k] = v[k];
-}
+    for (int i = lane / kShare; i < kPieces; i += 32 / kShare) {
+      const int t = i / (G::kN / 4), n4 = i % (G::kN / 4), q = n4 / kPer, piece = n4 % kPer, g0 = lane % kShare * kGroups;
+      f2 a = 0ull, b = 0ull;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&v[t][place((g0 + g) * G::kQ + q, piece)]);
+        a = g == 0 ? w.x : add2(a, w.x);
+        b = g == 0 ? w.y : add2(b, w.y);
+      }
+      float x[4];
+      unpack2(a, x[0], x[1]);
+      unpack2(b, x[2], x[3]);
+      if (kShare == 2)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] += __shfl_xor_sync(0xffffffffu, x[k], 1);
+      if (lane % kShare == 0) *reinterpret_cast<float4*>(out + t * out_row + n4 * 4) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+    __syncwarp();
+  }
+};
+template <typename G>
+struct GroupSums<G, false> {
+  // the token's sums of this lane's q go to out
+  __device__ __forceinline__ void put(int, int lane, const f2 (&s)[G::kPairs], float* out) {
+    float v[G::kNp];
+#pragma unroll
+    for (int p = 0; p < G::kPairs; ++p) unpack2(s[p], v[2 * p], v[2 * p + 1]);
+    int at = 0, left = G::kNp;
+#pragma unroll
+    for (int bit = 16; bit >= G::kQ; bit >>= 1) {
+      const bool up = lane & bit;
+      if (left > 1) {
+        left /= 2;
+#pragma unroll
+        for (int k = 0; k < left; ++k) v[k] = (up ? v[left + k] : v[k]) + __shfl_xor_sync(0xffffffffu, up ? v[k] : v[left + k], bit);
+        at += up ? left : 0;
+      } else {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);     // both hold the sum
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < left; ++k) out[at + k] = v[k];
+  }
+  __device__ __forceinline__ void take(int, float*, int) const {}
+};
 
 // a token's decays, and its step of the states
 template <typename G>
@@ -220,6 +259,10 @@ __device__ __forceinline__ void advance(const f2 (&e)[G::kCh][G::kPairs], const 
 #pragma unroll
     for (int p = 0; p < G::kPairs; ++p) h[c][p] = fma2(e[c][p], h[c][p], in[c][p]);
 }
+
+// CTAs of the backward kernel on an SM: sixteen states a lane need 168 registers to stay out of local memory (four CTAs of 128: 12% slower)
+template <typename G>
+constexpr int kBwdBlocks = G::kNp * G::kCh == 16 ? 3 : 4;
 
 // where a warp stands
 template <typename G>
@@ -439,8 +482,8 @@ __device__ __forceinline__ float at(const float4& v, int k) { return k == 0 ? v.
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 template <typename T, typename G>
-struct FwdSmem {
-  static constexpr int kT = 16;
+struct alignas(16) FwdSmem {
+  static constexpr int kT = G::kRows <= 8 ? 8 : 16;   // tokens of a tile: one access per tensor at least
   Raw<T, G, kT, 3> raw[2];
   float delta[kT][G::kWc], u[kT][G::kWc];
   float bc[2][kT][G::kN];
@@ -527,16 +570,17 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
       __syncwarp();
 #pragma unroll
       for (int half = 0; half < kT; half += kCkpt) {
-        const int todo = min(live, end) - t0;
-        if (half == 8 && todo > 8) {
+        const int at0 = kRev ? kT - kCkpt - half : half, from = t0 + at0, lim = min(live, end);   // tokens from .. from + 7
+        // the middle of 16 tokens (counted from the sequence's start, so that the way back meets the same states)
+        if (kRev ? from % 16 == 0 && from + kCkpt < lim : from % 16 != 0 && from < lim) {
           float two[G::kCh], more[G::kCh];
-          load_channels<G::kCh>(&s.delta[3][w.cg * G::kCh], two);
-          load_channels<G::kCh>(&s.delta[11][w.cg * G::kCh], more);
+          load_channels<G::kCh>(&s.delta[at0 + 1][w.cg * G::kCh], two);
+          load_channels<G::kCh>(&s.delta[at0 + 5][w.cg * G::kCh], more);
 #pragma unroll
           for (int c = 0; c < G::kCh; ++c) two[c] += more[c];
-          make_up<G>(two, (float)min(kT, todo), A, h);
+          make_up<G>(two, (float)min(16, lim - from / 16 * 16), A, h);
         }
-        if (kOut && a.checkpoints != nullptr && half < todo && t0 + half > 0) store_kept(a, w, (t0 + half) / kCkpt, h);
+        if (kOut && a.checkpoints != nullptr && from < lim && from > 0) store_kept(a, w, from / kCkpt, h);
 #pragma unroll 1
         for (int j0 = half; j0 < half + kCkpt; j0 += 4) {
         float own[4];
@@ -635,7 +679,7 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
 // reaches 32 of its lanes, one access moves a lane's 16 states, and 128 columns a CTA let four CTAs share an SM.  Kept in
 // registers they cost all occupancy, in shared memory 4 KB of traffic per token and warp.
 template <typename T, typename G>
-struct BwdWarpSmem {
+struct alignas(16) BwdWarpSmem {            // one behind the other for the CTA's warps
   static constexpr int kT = kCkpt;
   static constexpr int kBuf = sizeof(T) == 2 ? 2 : 1;
   Raw<T, G, kT, 4> raw[kBuf];
@@ -643,6 +687,7 @@ struct BwdWarpSmem {
   float inner[kT][G::kWc], through[kT][G::kWc], into[kT][G::kWc];
   float bc[2][kT][G::kN];
   float part[kT][2][G::kN];
+  GroupSums<G> sums;
 };
 
 // a lane's 8 or 16 floats to and from its row of tensor memory
@@ -693,11 +738,14 @@ __device__ __forceinline__ void tmem_fetched(uint32_t (&r)[16], f2 (&h)[G::kCh][
 __device__ __forceinline__ void tmem_kept_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <typename T, typename G>
-__global__ void __launch_bounds__(32 * kBwdWarps, 4)
+__global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks<G>)
 float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nseg, int seg_len, const float* sums, float* part_bc, float* part_grad,
                       Vec vec) {
   using S = BwdWarpSmem<T, G>;
+  static_assert(sizeof(S) % 16 == 0 && offsetof(S, delta) % 16 == 0 && offsetof(S, bc) % 16 == 0 && offsetof(S, part) % 16 == 0 && offsetof(S, sums) % 16 == 0,
+                "16-byte accesses");
   constexpr int kT = S::kT, kBuf = S::kBuf, kNp = G::kNp, kStates = G::kCh * kNp, kColumns = kT * kStates;
+  constexpr int kTurn = G::kNp == 16 ? 4 : kT;           // tokens between two GroupSums::take
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ uint32_t s_tmem;
   const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
@@ -813,91 +861,95 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
     widen_bc<T, G, kT>(raw, s.bc, t0, lim, a.dstate, lane);
     __syncwarp();
     // forward: C . h, and dC's sums over the warp's channels
+#pragma unroll 1
+    for (int turn = 0; turn < kT; turn += kTurn) {
 #pragma unroll 2
-    for (int t = 0; t < kT; ++t) {
-      float d[G::kCh], u[G::kCh], g[G::kCh], y[G::kCh], v[kNp];
-      f2 b2[G::kPairs], c2[G::kPairs], sC[G::kPairs], acc[G::kCh], e[G::kCh][G::kPairs];
-      load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
-      decays<G>(d, A, e);
-      load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
-      load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
-      load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
-      load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
-      tmem_keep<G>(tmem + t * kStates, h);
-      advance<G>(e, u, b2, h);
+      for (int t = turn; t < turn + kTurn; ++t) {
+        float d[G::kCh], u[G::kCh], g[G::kCh], y[G::kCh];
+        f2 b2[G::kPairs], c2[G::kPairs], sC[G::kPairs], acc[G::kCh], e[G::kCh][G::kPairs];
+        load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
+        decays<G>(d, A, e);
+        load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
+        load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
+        load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
+        load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
+        tmem_keep<G>(tmem + t * kStates, h);
+        advance<G>(e, u, b2, h);
 #pragma unroll
-      for (int p = 0; p < G::kPairs; ++p)
+        for (int p = 0; p < G::kPairs; ++p)
+#pragma unroll
+          for (int c = 0; c < G::kCh; ++c) {
+            acc[c] = p == 0 ? mul2(h[c][0], c2[0]) : fma2(h[c][p], c2[p], acc[c]);
+            sC[p] = c == 0 ? mul2(pack2(g[0], g[0]), h[0][p]) : fma2(pack2(g[c], g[c]), h[c][p], sC[p]);
+          }
 #pragma unroll
         for (int c = 0; c < G::kCh; ++c) {
-          acc[c] = p == 0 ? mul2(h[c][0], c2[0]) : fma2(h[c][p], c2[p], acc[c]);
-          sC[p] = c == 0 ? mul2(pack2(g[0], g[0]), h[0][p]) : fma2(pack2(g[c], g[c]), h[c][p], sC[p]);
+          float lo, hi;
+          unpack2(acc[c], lo, hi);
+          y[c] = lo + hi;
         }
-#pragma unroll
-      for (int c = 0; c < G::kCh; ++c) {
-        float lo, hi;
-        unpack2(acc[c], lo, hi);
-        y[c] = lo + hi;
+        const float own = own_channel<G::kCh, G::kQ>(y, w.q);
+        if (w.q % (G::kQ / G::kCh) == 0) s.inner[t][w.own] = own;
+        s.sums.put(t % 4, lane, sC, &s.part[t][1][w.q * kNp]);
       }
-      const float own = own_channel<G::kCh, G::kQ>(y, w.q);
-      if (w.q % (G::kQ / G::kCh) == 0) s.inner[t][w.own] = own;
-#pragma unroll
-      for (int p = 0; p < G::kPairs; ++p) unpack2(sC[p], v[2 * p], v[2 * p + 1]);
-      over_groups<kNp, G::kQ>(v, lane, &s.part[t][1][w.q * kNp]);
+      s.sums.take(lane, &s.part[turn][1][0], 2 * G::kN);
     }
     tmem_kept_wait();
     // and back
+#pragma unroll 1
+    for (int turn = kT - kTurn; turn >= 0; turn -= kTurn) {
 #pragma unroll 2
-    for (int t = kT - 1; t >= 0; --t) {
-      float d[G::kCh], u[G::kCh], g[G::kCh], through[G::kCh], into[G::kCh], v[kNp];
-      f2 b2[G::kPairs], c2[G::kPairs], sB[G::kPairs], e[G::kCh][G::kPairs], dh[G::kCh][G::kPairs], thr[G::kCh], q2[G::kCh];
-      uint32_t kept[16];
-      tmem_fetch<G>(tmem + t * kStates, kept);
-      load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
-      decays<G>(d, A, e);
-      load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
-      load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
-      load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
-      load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
+      for (int t = turn + kTurn - 1; t >= turn; --t) {
+        float d[G::kCh], u[G::kCh], g[G::kCh], through[G::kCh], into[G::kCh];
+        f2 b2[G::kPairs], c2[G::kPairs], sB[G::kPairs], e[G::kCh][G::kPairs], dh[G::kCh][G::kPairs], thr[G::kCh], q2[G::kCh];
+        uint32_t kept[16];
+        tmem_fetch<G>(tmem + t * kStates, kept);
+        load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
+        decays<G>(d, A, e);
+        load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
+        load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
+        load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
+        load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
 #pragma unroll
-      for (int c = 0; c < G::kCh; ++c)
+        for (int c = 0; c < G::kCh; ++c)
 #pragma unroll
-        for (int p = 0; p < G::kPairs; ++p) dh[c][p] = fma2(c2[p], pack2(g[c], g[c]), carry[c][p]);
+          for (int p = 0; p < G::kPairs; ++p) dh[c][p] = fma2(c2[p], pack2(g[c], g[c]), carry[c][p]);
 #pragma unroll
-      for (int c = 0; c < G::kCh; ++c)
+        for (int c = 0; c < G::kCh; ++c)
 #pragma unroll
-        for (int p = 0; p < G::kPairs; ++p) carry[c][p] = mul2(dh[c][p], e[c][p]);
+          for (int p = 0; p < G::kPairs; ++p) carry[c][p] = mul2(dh[c][p], e[c][p]);
 #pragma unroll
-      for (int p = 0; p < G::kPairs; ++p)
+        for (int p = 0; p < G::kPairs; ++p)
+#pragma unroll
+          for (int c = 0; c < G::kCh; ++c) {
+            sB[p] = c == 0 ? mul2(pack2(u[0], u[0]), dh[0][p]) : fma2(pack2(u[c], u[c]), dh[c][p], sB[p]);
+            thr[c] = p == 0 ? mul2(dh[c][0], b2[0]) : fma2(dh[c][p], b2[p], thr[c]);
+          }
+        tmem_fetched<G>(kept, h);
+#pragma unroll
+        for (int p = 0; p < G::kPairs; ++p)
+#pragma unroll
+          for (int c = 0; c < G::kCh; ++c) {
+            dh[c][p] = mul2(carry[c][p], h[c][p]);
+            q2[c] = p == 0 ? mul2(dh[c][0], A[c][0]) : fma2(dh[c][p], A[c][p], q2[c]);
+            dA[c][p] = fma2(dh[c][p], pack2(d[c], d[c]), dA[c][p]);
+          }
 #pragma unroll
         for (int c = 0; c < G::kCh; ++c) {
-          sB[p] = c == 0 ? mul2(pack2(u[0], u[0]), dh[0][p]) : fma2(pack2(u[c], u[c]), dh[c][p], sB[p]);
-          thr[c] = p == 0 ? mul2(dh[c][0], b2[0]) : fma2(dh[c][p], b2[p], thr[c]);
+          float lo, hi;
+          unpack2(thr[c], lo, hi);
+          through[c] = lo + hi;
+          unpack2(q2[c], lo, hi);
+          into[c] = lo + hi;
         }
-      tmem_fetched<G>(kept, h);
-#pragma unroll
-      for (int p = 0; p < G::kPairs; ++p)
-#pragma unroll
-        for (int c = 0; c < G::kCh; ++c) {
-          dh[c][p] = mul2(carry[c][p], h[c][p]);
-          q2[c] = p == 0 ? mul2(dh[c][0], A[c][0]) : fma2(dh[c][p], A[c][p], q2[c]);
-          dA[c][p] = fma2(dh[c][p], pack2(d[c], d[c]), dA[c][p]);
+        s.sums.put(t % 4, lane, sB, &s.part[t][0][w.q * kNp]);
+        const float own_through = own_channel<G::kCh, G::kQ>(through, w.q), own_into = own_channel<G::kCh, G::kQ>(into, w.q);
+        if (w.q % (G::kQ / G::kCh) == 0) {
+          s.through[t][w.own] = own_through;
+          s.into[t][w.own] = own_into;
         }
-#pragma unroll
-      for (int c = 0; c < G::kCh; ++c) {
-        float lo, hi;
-        unpack2(thr[c], lo, hi);
-        through[c] = lo + hi;
-        unpack2(q2[c], lo, hi);
-        into[c] = lo + hi;
       }
-#pragma unroll
-      for (int p = 0; p < G::kPairs; ++p) unpack2(sB[p], v[2 * p], v[2 * p + 1]);
-      over_groups<kNp, G::kQ>(v, lane, &s.part[t][0][w.q * kNp]);
-      const float own_through = own_channel<G::kCh, G::kQ>(through, w.q), own_into = own_channel<G::kCh, G::kQ>(into, w.q);
-      if (w.q % (G::kQ / G::kCh) == 0) {
-        s.through[t][w.own] = own_through;
-        s.into[t][w.own] = own_into;
-      }
+      s.sums.take(lane, &s.part[turn][0][0], 2 * G::kN);
     }
     if (chunk % 2 == 1) {                                // the middle of a tile of the forward pass
       float two[G::kCh], more[G::kCh];
@@ -1018,61 +1070,107 @@ __global__ void __launch_bounds__(G::kGrad) float_scan_param_kernel(const __grid
 }
 
 // ---- one token --------------------------------------------------------------------------------------------------------------
-// Bound by the state, read and written once (8 bytes per state).  kLanes lanes of a channel hold four states each.
+// Bound by the state, read and written once (8 bytes per state).  kLanes lanes of a channel hold four states each and walk `rows`
+// sequences, kAhead at a time: all loads first, so that enough is under way.  What a (sequence, channel) costs besides its
+// states -- loads, softplus, gate, output -- a lane does for its own share of the kAhead sequences only, and passes delta and delta x round.
+constexpr int kAhead = 4;
 template <typename T, int kLanes>
-__global__ void __launch_bounds__(128) float_update_kernel(const __grid_constant__ qb_float_update_args a, int vec) {
-  const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-  const int sub = (int)(i % kLanes), n0 = sub * 4;
-  const int64_t bd = min(i / kLanes, (int64_t)a.batch * a.dim - 1);      // the last lanes repeat the last channel, for the shuffles
-  const bool mine = i / kLanes == bd;
-  const int b = (int)(bd / a.dim), d = (int)(bd % a.dim), g = d / (a.dim / a.groups);
-  const float* st = a.state + b * a.state_sb + (int64_t)d * a.state_sd + n0;
-  float h[4], A[4], B[4], C[4];
-  if (vec) {
-    const float4 v = n0 < a.dstate ? *reinterpret_cast<const float4*>(st) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
-  }
-  const T* Bp = static_cast<const T*>(a.Bm) + b * a.B_sb + (int64_t)g * a.B_sg + n0;
-  const T* Cp = static_cast<const T*>(a.Cm) + b * a.C_sb + (int64_t)g * a.C_sg + n0;
+__global__ void __launch_bounds__(128, 6) float_update_kernel(const __grid_constant__ qb_float_update_args a, int rows, int vec, int vec_bc) {
+  constexpr int kOwners = kLanes < kAhead ? kLanes : kAhead, kOwn = kAhead / kOwners;
+  const int i = (int)blockIdx.x * 128 + (int)threadIdx.x;
+  const int sub = i % kLanes, n0 = sub * 4, d = min(i / kLanes, a.dim - 1), g = d / (a.dim / a.groups);   // the last lanes repeat the last channel
+  const bool mine = i / kLanes == d;
+  f2 A[2];
+  {
+    float v[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const bool in = n0 + k < a.dstate;
-    if (!vec) h[k] = in ? st[k] : 0.0f;
-    A[k] = in ? a.A[(int64_t)d * a.dstate + n0 + k] * kLog2e : 0.0f;
-    B[k] = in ? to_f(Bp[k]) : 0.0f;
-    C[k] = in ? to_f(Cp[k]) : 0.0f;
+    for (int k = 0; k < 4; ++k) v[k] = n0 + k < a.dstate ? a.A[(int64_t)d * a.dstate + n0 + k] * kLog2e : 0.0f;
+    A[0] = pack2(v[0], v[1]);
+    A[1] = pack2(v[2], v[3]);
   }
-  const float x = to_f(static_cast<const T*>(a.x)[b * a.x_sb + d]);
-  float dl = to_f(static_cast<const T*>(a.dt)[b * a.dt_sb + d]) + (a.dt_bias != nullptr ? a.dt_bias[d] : 0.0f);
-  if (a.dt_softplus) {
-    float twin = dl;
-    softplus_series(dl, twin);
-  }
-  const float u = dl * x;
-  float y = 0.0f;
+  const float bias = a.dt_bias != nullptr ? a.dt_bias[d] : 0.0f, Dv = a.D != nullptr ? a.D[d] : 0.0f;
+  const int b0 = (int)blockIdx.y * rows, b1 = min(a.batch, b0 + rows), own0 = min(sub, kOwners - 1) * kOwn;
+  const float* st = a.state + b0 * a.state_sb + (int64_t)d * a.state_sd + n0;
+  float* so = a.state_out + b0 * a.state_out_sb + (int64_t)d * a.state_out_sd + n0;
+  const T* Bp = static_cast<const T*>(a.Bm) + b0 * a.B_sb + (int64_t)g * a.B_sg + n0;
+  const T* Cp = static_cast<const T*>(a.Cm) + b0 * a.C_sb + (int64_t)g * a.C_sg + n0;
+  for (int c0 = b0; c0 < b1; c0 += kAhead) {
+    float4 h[kAhead], B[kAhead], C[kAhead];
+    float x[kOwn], dl[kOwn], z[kOwn], u[kOwn], own_y[kOwn];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    h[k] = fmaf(exp2_series(dl * A[k]), h[k], u * B[k]);   // one decay a call: see make_up()
-    y = fmaf(h[k], C[k], y);
-  }
-#pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (!mine) return;
-  float* so = a.state_out + b * a.state_out_sb + (int64_t)d * a.state_out_sd + n0;
-  if (vec) {
-    if (n0 < a.dstate) *reinterpret_cast<float4*>(so) = make_float4(h[0], h[1], h[2], h[3]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (n0 + k < a.dstate) so[k] = h[k];
-  }
-  if (sub == 0) {
-    if (a.D != nullptr) y = fmaf(a.D[d], x, y);
-    if (a.z != nullptr) {
-      const float z = to_f(static_cast<const T*>(a.z)[b * a.z_sb + d]);
-      y *= z * sigmoid_fast(z);
+    for (int k = 0; k < kOwn; ++k) {
+      const int64_t b = min(c0 + own0 + k, b1 - 1);      // past the last: the last again
+      x[k] = to_f(static_cast<const T*>(a.x)[b * a.x_sb + d]);
+      dl[k] = to_f(static_cast<const T*>(a.dt)[b * a.dt_sb + d]);
+      z[k] = a.z != nullptr ? to_f(static_cast<const T*>(a.z)[b * a.z_sb + d]) : 0.0f;
     }
-    static_cast<T*>(a.y)[(int64_t)b * a.dim + d] = from_f<T>(y);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      h[k] = B[k] = C[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (c0 + k < b1) {
+        if (vec) {
+          if (n0 < a.dstate) h[k] = *reinterpret_cast<const float4*>(st);
+        } else {
+          if (n0 < a.dstate) h[k].x = st[0];
+          if (n0 + 1 < a.dstate) h[k].y = st[1];
+          if (n0 + 2 < a.dstate) h[k].z = st[2];
+          if (n0 + 3 < a.dstate) h[k].w = st[3];
+        }
+        if (vec_bc) {
+          if (n0 < a.dstate) { B[k] = quad(Bp); C[k] = quad(Cp); }
+        } else {
+          if (n0 < a.dstate) { B[k].x = to_f(Bp[0]); C[k].x = to_f(Cp[0]); }
+          if (n0 + 1 < a.dstate) { B[k].y = to_f(Bp[1]); C[k].y = to_f(Cp[1]); }
+          if (n0 + 2 < a.dstate) { B[k].z = to_f(Bp[2]); C[k].z = to_f(Cp[2]); }
+          if (n0 + 3 < a.dstate) { B[k].w = to_f(Bp[3]); C[k].w = to_f(Cp[3]); }
+        }
+      }
+      st += a.state_sb;
+      Bp += a.B_sb;
+      Cp += a.C_sb;
+    }
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      dl[k] += bias;
+      float twin = dl[k];
+      if (a.dt_softplus) softplus_series(dl[k], twin);
+      u[k] = dl[k] * x[k];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      // one decay a call: what is systematic in it would add up over calls (see make_up())
+      const f2 dd = splat(__shfl_sync(0xffffffffu, dl[k % kOwn], k / kOwn, kLanes)), uu = splat(__shfl_sync(0xffffffffu, u[k % kOwn], k / kOwn, kLanes));
+      const f2 h0 = fma2(exp2_fine(mul2(dd, A[0])), pack2(h[k].x, h[k].y), mul2(uu, pack2(B[k].x, B[k].y)));
+      const f2 h1 = fma2(exp2_fine(mul2(dd, A[1])), pack2(h[k].z, h[k].w), mul2(uu, pack2(B[k].z, B[k].w)));
+      float y, y1;
+      unpack2(fma2(h1, pack2(C[k].z, C[k].w), mul2(h0, pack2(C[k].x, C[k].y))), y, y1);
+      y += y1;
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (k / kOwn == min(sub, kOwners - 1)) own_y[k % kOwn] = y;
+      if (mine && c0 + k < b1) {
+        float4 r;
+        unpack2(h0, r.x, r.y);
+        unpack2(h1, r.z, r.w);
+        if (vec) {
+          if (n0 < a.dstate) *reinterpret_cast<float4*>(so) = r;
+        } else {
+          if (n0 < a.dstate) so[0] = r.x;
+          if (n0 + 1 < a.dstate) so[1] = r.y;
+          if (n0 + 2 < a.dstate) so[2] = r.z;
+          if (n0 + 3 < a.dstate) so[3] = r.w;
+        }
+      }
+      so += a.state_out_sb;
+    }
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const int b = c0 + own0 + k;
+      float y = own_y[k];
+      if (a.D != nullptr) y = fmaf(Dv, x[k], y);
+      if (a.z != nullptr) y *= z[k] * sigmoid_fast(z[k]);
+      if (mine && b < b1 && sub < kOwners) static_cast<T*>(a.y)[(int64_t)b * a.dim + d] = from_f<T>(y);
+    }
   }
 }
 
@@ -1118,7 +1216,7 @@ Plan plan_bwd(int batch, int seqlen, int dim, int groups, int dstate) {
   const int64_t sms = sm_count();
   Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 2, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 2, 4) : share_of(batch, dim, groups, 16, 1, 4);
   if (p.ch == 2 && (int64_t)batch * p.tiles < 4 * sms) p = share_of(batch, dim, groups, 8, 1, p.q);
-  const int64_t ctas = std::max<int64_t>(1, (int64_t)batch * groups * ceil_div(p.tpg, kBwdWarps)), slots = 4 * sms;
+  const int64_t ctas = std::max<int64_t>(1, (int64_t)batch * groups * ceil_div(p.tpg, kBwdWarps)), slots = (p.np == 16 ? 2 : p.ch == 2 ? 3 : 4) * sms;
   int64_t best = 1;
   double least = 0.0;
   for (int64_t n = 1; n <= std::min<int64_t>(24, std::max(1, seqlen / kMinSeg)); ++n) {
@@ -1297,20 +1395,25 @@ extern "C" int qb_float_scan_update(const qb_float_update_args* a, void* stream)
   QB_REQUIRE(a->dtype >= 0 && a->dtype <= 2, QB_ERR_INVALID_ARG, "float_scan_update: unsupported type");
   if (a->batch == 0) return QB_OK;
   const int lanes = a->dstate <= 4 ? 1 : a->dstate <= 8 ? 2 : a->dstate <= 16 ? 4 : a->dstate <= 32 ? 8 : 16;
-  const int64_t grid = ceil_div((int64_t)a->batch * a->dim * lanes, 128);
-  QB_REQUIRE(grid < (1ll << 31), QB_ERR_TOO_LARGE, "float_scan_update: batch and dim are too large");
+  const int64_t across = ceil_div((int64_t)a->dim * lanes, 128);
+  // sequences of a thread: as many as leave every SM six CTAs, in whole turns of kAhead (64 x 5120 x 16 states: 17 us, one each 37)
+  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(a->batch, ceil_div(across * a->batch, 6 * sm_count())));
+  const int64_t rows = share > 2 ? ceil_div(share, kAhead) * kAhead : share, down = ceil_div(a->batch, rows);
+  QB_REQUIRE(across < (1ll << 31) && down < 65536, QB_ERR_TOO_LARGE, "float_scan_update: batch and dim are too large");
+  const size_t size = a->dtype == 0 ? 4 : 2;
   const int vec = a->dstate % 4 == 0 && aligned(a->state, 16) && aligned(a->state_out, 16) &&
                   (a->state_sb | a->state_sd | a->state_out_sb | a->state_out_sd) % 4 == 0;
+  const int vec_bc = a->dstate % 4 == 0 && aligned(a->Bm, 4 * size) && aligned(a->Cm, 4 * size) && (a->B_sb | a->B_sg | a->C_sb | a->C_sg) % 4 == 0;
   return by_type(a->dtype, [&](auto t) -> int {
     using T = decltype(t);
     cudaStream_t st = (cudaStream_t)stream;
-    const unsigned g = (unsigned)grid;
+    const dim3 g((unsigned)across, (unsigned)down);
     switch (lanes) {
-      case 1: float_update_kernel<T, 1><<<g, 128, 0, st>>>(*a, vec); break;
-      case 2: float_update_kernel<T, 2><<<g, 128, 0, st>>>(*a, vec); break;
-      case 4: float_update_kernel<T, 4><<<g, 128, 0, st>>>(*a, vec); break;
-      case 8: float_update_kernel<T, 8><<<g, 128, 0, st>>>(*a, vec); break;
-      default: float_update_kernel<T, 16><<<g, 128, 0, st>>>(*a, vec);
+      case 1: float_update_kernel<T, 1><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc); break;
+      case 2: float_update_kernel<T, 2><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc); break;
+      case 4: float_update_kernel<T, 4><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc); break;
+      case 8: float_update_kernel<T, 8><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc); break;
+      default: float_update_kernel<T, 16><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc);
     }
     QB_LAUNCH_OK("float_update_kernel");
     return QB_OK;
