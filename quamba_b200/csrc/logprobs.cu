@@ -7,12 +7,18 @@
 // leaves at the memory's speed.  Many rows take a CTA each; few rows a cluster of up to eight, whose parts are joined over
 // distributed shared memory.
 //
-// Alternatives in the same pass.  The maxima of 128 groups of a CTA's threads over their first four pieces are ranked: the top_k-th of
+// Alternatives in the same pass.  The maxima of 64 groups of a CTA's threads over their first four pieces are ranked: the top_k-th of
 // them is a bound that at least top_k values reach, so what is below it never counts again.  Values that reach it are listed
 // (some tens), and the list is ranked at the end by (value, column).  A list that runs over (long plateaus of equal
-// values, rows that rise to the end) sends the row's part to top_k searches for the largest key below the last.
+// values, rows that rise to the end) sends the row's part to top_k searches for the largest key below the last.  A cluster's
+// lists, each in order, are merged by bisection.
 //
-// Bound by the row's bytes: read once forward; read and written once backward.
+// Bound by the row's bytes, read once forward; read and written once backward: 8192 x 50280 fp16 128 us (6.5 TB/s), with the
+// entropy 136; 4096 x 50288 bf16 with the entropy 75 us (5.5) and 149 us (5.5) back; 4096 x 50288 fp32 122 us (6.8) and 252 us.
+// With alternatives by the phases between a CTA's barriers as well, of which three CTAs hide too little: 198 us for five of
+// 8192 x 50280 fp16, 253 for twenty and the entropy.  Few rows are a chain of latencies: 8 x 50280 fp16 3.4 us, 6.8 with twenty
+// alternatives and the entropy (first loads 1.0, bound 0.5, second reading 1.0, joining and ranking 1.2, cluster barrier 0.9, merging
+// and answering 1.3).
 #include <algorithm>
 #include "common.cuh"
 
@@ -24,7 +30,7 @@ namespace {
 
 constexpr int kStatusTarget = 502;       // keep in step with qb_read_device_status (lib.cu)
 constexpr int kMaxCluster = 8;
-constexpr int kMaxGroups = 128;          // groups of threads whose first maxima are ranked
+constexpr int kGroups = 64;              // groups of threads whose first maxima are ranked (128: as many candidates, twice the time)
 constexpr int kList = 2048;              // candidates listed per CTA
 constexpr int kTop = QB_LOGPROBS_MAX_TOP;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -81,6 +87,19 @@ __device__ __forceinline__ Stats join(Stats x, Stats y) {
   if (x.m != m) raise(x, m);               // a side without numbers (m = -inf) has s = w = 0, or a NaN
   if (y.m != m) raise(y, m);
   return Stats{m, x.s + y.s, x.w + y.w};
+}
+// a warp's, in every lane
+__device__ __forceinline__ Stats join_warp(Stats x) {
+  float m = x.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (x.m != m) raise(x, m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    x.s += __shfl_xor_sync(0xffffffffu, x.s, o);
+    x.w += __shfl_xor_sync(0xffffffffu, x.w, o);
+  }
+  return x;
 }
 template <bool kEntropy>
 __device__ __forceinline__ void add_one(Stats& a, float x) {
@@ -141,6 +160,12 @@ struct Part {
   __device__ __forceinline__ int single(int i) const { return i < head ? begin + i : begin + i + body * Wide<T>::kN; }
 };
 
+// where row r begins (there are fewer than 2^31 rows, and a 64-bit division would hold a CTA's first load up)
+__device__ __forceinline__ int64_t row_at(const qb_logprobs_args& a, uint32_t r, int64_t outer, int64_t inner) {
+  const uint32_t n = (uint32_t)min(a.inner_rows, (int64_t)0x7fffffff), o = r / n;
+  return o * outer + (r - o * n) * inner;
+}
+
 // the cluster's first CTA's copy of a shared variable (its own where there is no cluster)
 template <typename V>
 __device__ __forceinline__ V* cluster_first(V* mine) {
@@ -151,7 +176,7 @@ __device__ __forceinline__ V* cluster_first(V* mine) {
 
 // Selecting the top_k of a part.
 struct Select {
-  float group[kMaxGroups];
+  uint32_t group[kGroups];
   uint64_t list[kList];
   uint64_t best[kMaxCluster * kTop];       // the winners of the cluster's CTAs, in the first one
   uint64_t warp_key[32];
@@ -159,32 +184,42 @@ struct Select {
   float bound;
 };
 
-// the top_k-th largest of n floats in shared memory becomes *bound, for n <= blockDim.x
-__device__ __forceinline__ void kth_of(const float* v, int n, int top_k, float* bound) {
-  if ((int)threadIdx.x >= n) return;
-  const float mine = v[threadIdx.x];
-  int above = 0, reach = 0;
-  for (int j = 0; j < n; j += 4) {
-    const float4 q = *reinterpret_cast<const float4*>(v + j);
+// A number that at least top_k of kGroups floats reach: the top_k-th largest, or for fp32 up to 2^-17 less, since the low bits
+// of the order-preserving keys give way to the place, which makes them all different.
+__device__ __forceinline__ uint32_t place_key(float v, int at) { return (rank_of(v) & ~(uint32_t)(kGroups - 1)) | (uint32_t)at; }
+__device__ __forceinline__ void bound_of(const uint32_t* keys, int top_k, float* bound) {
+  const int tid = (int)threadIdx.x;
+  if (tid >= kGroups) return;
+  const uint32_t mine = keys[tid];
+  int above = 0;
+#pragma unroll 4
+  for (int j = 0; j < kGroups; j += 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(keys + j);
     above += (q.x > mine) + (q.y > mine) + (q.z > mine) + (q.w > mine);
-    reach += (q.x >= mine) + (q.y >= mine) + (q.z >= mine) + (q.w >= mine);
   }
-  if (above < top_k && reach >= top_k) *bound = mine;      // equal values pass together and write the same
+  if (above == top_k - 1) *bound = value_of((uint64_t)max(mine & ~(uint32_t)(kGroups - 1), rank_of(neg_inf())) << 32);
 }
 
+// Without alternatives six CTAs of 256 threads an SM (40 registers): 8192 x 50280 fp16 131 us, where the five that 48 registers
+// leave take 140; with the entropy 4096 x 50288 bf16 79 us against 89 at four.  Eight, or four rows of 16 bytes ahead made two,
+// are no faster.
 template <typename T, int kThreads, bool kEntropy, bool kAlt>
-__global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) logprobs_kernel(const __grid_constant__ qb_logprobs_args a, int parts, int part_len, int* status) {
-  constexpr int kWarps = kThreads / 32, kN = Wide<T>::kN, kAhead = 4, kGroups = kThreads < kMaxGroups ? kThreads : kMaxGroups;
+__global__ void __launch_bounds__(kThreads, kThreads == 64 ? 1 : kAlt ? 3 : 6) logprobs_kernel(const __grid_constant__ qb_logprobs_args a, int parts, int part_len, int* status) {
+  constexpr int kWarps = kThreads / 32, kN = Wide<T>::kN, kAhead = 4;
   __shared__ Stats s_stats[kWarps], s_parts[kMaxCluster];
   __shared__ __align__(16) unsigned char s_select[kAlt ? sizeof(Select) : 16];
   Select& sel = *reinterpret_cast<Select*>(s_select);
   const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = (int)(blockIdx.x % parts);           // the cluster is `parts` neighbouring CTAs
-  const int64_t r = blockIdx.x / parts;
-  const T* const row = static_cast<const T*>(a.logits) + r / a.inner_rows * a.outer_stride + r % a.inner_rows * a.row_stride;
+  const int rank = (int)(blockIdx.x % (uint32_t)parts);           // the cluster is `parts` neighbouring CTAs
+  const uint32_t r = blockIdx.x / (uint32_t)parts;
+  const T* const row = static_cast<const T*>(a.logits) + row_at(a, r, a.outer_stride, a.row_stride);
   const int from = rank * part_len, to = min(a.vocab, from + part_len);
   const Part<T> part(row, min(from, a.vocab), max(to, min(from, a.vocab)));
 
+  const bool teller = tid == kThreads - 32 && rank == 0;   // not in the first warp: that one has alternatives to rank
+  // asked for before the row and its value while the sums are joined: 128 us against 131 at 8192 x 50280 fp16, 3.4 against 3.7 at 8
+  // rows; beside the alternatives' registers it costs more than it gives
+  int64_t target = !kAlt && teller ? a.targets[r] : -1;
   if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   Stats st{neg_inf(), 0.0f, 0.0f};
   f2 s2 = 0ull, w2 = 0ull;
@@ -196,9 +231,14 @@ __global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) log
     }
   };
   const auto look = [&](const Wide<T>& v, float top, int c) {
-    if (top >= bound)
+    if (!(top >= bound)) return;
+    unsigned which = 0;
 #pragma unroll
-      for (int k = 0; k < kN; ++k) list_it(val(v.v[k]), c + k);
+    for (int k = 0; k < kN; ++k) which |= val(v.v[k]) >= bound ? 1u << k : 0u;
+    for (; which != 0; which &= which - 1) {             // one, as a rule; read again, which keeps this short code that rarely runs
+      const int k = __ffs((int)which) - 1;
+      list_it(val(row[c + k]), c + k);
+    }
   };
   int i = tid;
   if (kAlt) {
@@ -207,9 +247,9 @@ __global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) log
     for (int j = tid; j < min(part.body, kAhead * kThreads); j += kThreads) over = fmaxf(over, largest(load16(row + part.piece(j))));
 #pragma unroll
     for (int o = kThreads / kGroups / 2; o > 0; o /= 2) over = fmaxf(over, __shfl_xor_sync(0xffffffffu, over, o));
-    if (tid % (kThreads / kGroups) == 0) sel.group[tid / (kThreads / kGroups)] = over;
+    if (tid % (kThreads / kGroups) == 0) sel.group[tid / (kThreads / kGroups)] = place_key(over, tid / (kThreads / kGroups));
     __syncthreads();
-    kth_of(sel.group, kGroups, a.top_k, &sel.bound);
+    bound_of(sel.group, a.top_k, &sel.bound);
     __syncthreads();
     bound = sel.bound;
   }
@@ -224,11 +264,23 @@ __global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) log
       if (kAlt) look(v[j], top, part.piece(i + j * kThreads));
     }
   }
-  for (; i < part.body; i += kThreads) {
-    const Wide<T> v = load16(row + part.piece(i));
-    const float top = largest(v);
-    add_piece<kEntropy>(st, s2, w2, v, top);
-    if (kAlt) look(v, top, part.piece(i));
+  if (kAlt) {                              // the last pieces, fewer than kAhead a thread: one by one where the code is long
+    for (; i < part.body; i += kThreads) {
+      const Wide<T> v = load16(row + part.piece(i));
+      const float top = largest(v);
+      add_piece<kEntropy>(st, s2, w2, v, top);
+      look(v, top, part.piece(i));
+    }
+  } else if (i < part.body) {
+    Wide<T> v[kAhead - 1];
+#pragma unroll
+    for (int j = 0; j < kAhead - 1; ++j)
+      if (i + j * kThreads < part.body) v[j] = load16(row + part.piece(i + j * kThreads));
+#pragma unroll
+    for (int j = 0; j < kAhead - 1; ++j) {
+      if (i + j * kThreads >= part.body) break;
+      add_piece<kEntropy>(st, s2, w2, v[j], largest(v[j]));
+    }
   }
   {
     float x, y;
@@ -243,19 +295,20 @@ __global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) log
     add_one<kEntropy>(st, x);
     if (kAlt) list_it(x, c);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    st = join(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.w, o)});
+  float given = 0.0f;
+  if (!kAlt && teller && target >= 0 && target < a.vocab) given = val(row[target]);
+  st = join_warp(st);
   if (lane == 0) s_stats[warp] = st;
   __syncthreads();
   // The first CTA runs: its shared memory may be written.  (None of the cluster barriers is the .aligned form: that one wants whole
   // warps at a time, and lanes leave the loops over listed keys below one by one.)
   if (parts > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 
-  if (kAlt) {                              // this part's best into sel.best[0 .. found), in no order
+  int found = 0;
+  if (kAlt) {                              // this part's best into the first CTA's sel.best, in order, zeros behind
     const int n = sel.count;
     uint64_t* const out = cluster_first(sel.best) + rank * kTop;
-    int found = min(n, a.top_k);
+    found = min(n, a.top_k);
     if (n <= kList) {
       for (int j = tid; j < n; j += kThreads) {
         const uint64_t mine = sel.list[j];
@@ -269,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) log
         uint64_t best = 0;
         const auto see = [&](float x, int c) {
           const uint64_t key = key_of(x, (uint32_t)c);
-          if (key < below && key > best) best = key;
+          if (x > neg_inf() && key < below && key > best) best = key;
         };
         for (int j = tid; j < part.body; j += kThreads) {
           const Wide<T> v = load16(row + part.piece(j));
@@ -288,54 +341,62 @@ __global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) log
       }
       found = a.top_k;                     // more than kList columns: there are as many
     }
+    if (tid >= found && tid < kTop) out[tid] = 0;
     if (tid == 0) cluster_first(sel.found)[rank] = found;
   }
-  if (warp == 0) {
-    st = lane < kWarps ? s_stats[lane] : Stats{neg_inf(), 0.0f, 0.0f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      st = join(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.w, o)});
-    if (lane == 0) cluster_first(s_parts)[rank] = st;
-  }
   if (parts > 1) {
+    if (warp == 0) {
+      st = join_warp(lane < kWarps ? s_stats[lane] : Stats{neg_inf(), 0.0f, 0.0f});
+      if (lane == 0) cluster_first(s_parts)[rank] = st;
+    }
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     if (rank != 0) return;
+    st = join_warp(lane < parts ? s_parts[lane] : Stats{neg_inf(), 0.0f, 0.0f});
   } else {
-    __syncthreads();
+    if (kAlt) __syncthreads();
+    st = join_warp(lane < kWarps ? s_stats[lane] : Stats{neg_inf(), 0.0f, 0.0f});
   }
-
-  st = s_parts[0];
-  for (int j = 1; j < parts; ++j) st = join(st, s_parts[j]);
   const bool empty = st.m == neg_inf() && st.s == 0.0f;
   const float logs = log2f(st.s);
   const auto logprob = [&](float x) { return empty ? neg_inf() : fmaf(-logs, kLn2, x - st.m); };
-  if (tid == 0) {
-    const int64_t t = a.targets[r];
+  if (teller) {
+    if (kAlt) target = a.targets[r];
+    const bool inside = target >= 0 && target < a.vocab;
+    if (kAlt && inside) given = val(row[target]);
     float lp = 0.0f;
-    if (t != a.ignore_index) {
-      if (t >= 0 && t < a.vocab) {
-        lp = logprob(val(row[t]));
-      } else {
-        lp = quiet_nan();
-        atomicCAS(status, 0, kStatusTarget);
-      }
+    if (target != a.ignore_index) {
+      lp = inside ? logprob(given) : quiet_nan();
+      if (!inside) atomicCAS(status, 0, kStatusTarget);
     }
     a.logprobs[r] = lp;
     if (kEntropy) a.entropy[r] = empty ? 0.0f : (logs - st.w / st.s) * kLn2;
     if (a.lse != nullptr) a.lse[r] = empty ? neg_inf() : fmaf(logs, kLn2, st.m);
   }
   if (kAlt) {
-    int n = 0;
-    for (int j = 0; j < parts; ++j) n += sel.found[j];
-    for (int j = tid; j < parts * kTop; j += kThreads) {
-      if (j % kTop >= sel.found[j / kTop]) continue;
-      const uint64_t mine = sel.best[j];
-      int above = 0;
-      for (int q = 0; q < parts; ++q)
-        for (int k = 0; k < sel.found[q]; ++k) above += sel.best[q * kTop + k] > mine;
-      if (above < a.top_k) {
-        a.top_ids[r * a.top_k + above] = column_of(mine);
-        a.top_logprobs[r * a.top_k + above] = logprob(value_of(mine));
+    const auto answer = [&](int at, uint64_t key) {
+      a.top_ids[(int64_t)r * a.top_k + at] = column_of(key);
+      a.top_logprobs[(int64_t)r * a.top_k + at] = logprob(value_of(key));
+    };
+    int n = found;
+    if (parts == 1) {
+      if (tid < found) answer(tid, sel.best[tid]);
+    } else {
+      n = 0;
+      for (int j = 0; j < parts; ++j) n += sel.found[j];
+      // a key's place: how many of each part's keys are above it, by bisection in all parts at once
+      for (int j = tid; j < parts * a.top_k; j += kThreads) {
+        const uint64_t mine = sel.best[j % parts * kTop + j / parts];
+        const uint64_t* at[kMaxCluster];   // the first key not known to be above
+        int place = 0;
+#pragma unroll
+        for (int q = 0; q < kMaxCluster; ++q) at[q] = sel.best + min(q, parts - 1) * kTop;
+#pragma unroll
+        for (int step = kTop / 2; step > 0; step /= 2)
+#pragma unroll
+          for (int q = 0; q < kMaxCluster; ++q) at[q] += at[q][step - 1] > mine ? step : 0;
+#pragma unroll
+        for (int q = 0; q < kMaxCluster; ++q) place += q < parts ? (int)(at[q] - (sel.best + q * kTop)) + (*at[q] > mine) : 0;
+        if (mine != 0 && place < a.top_k) answer(place, mine);
       }
     }
     // fewer numbers above -inf than asked for: the lowest of the other columns (-inf, or NaN in a row without a distribution)
@@ -343,22 +404,23 @@ __global__ void __launch_bounds__(kThreads, kAlt && kThreads == 512 ? 3 : 1) log
       for (int c = 0; c < a.vocab && n < a.top_k; ++c) {
         const float x = val(row[c]);
         if (x > neg_inf()) continue;
-        a.top_ids[r * a.top_k + n] = c;
-        a.top_logprobs[r * a.top_k + n] = logprob(x);
+        a.top_ids[(int64_t)r * a.top_k + n] = c;
+        a.top_logprobs[(int64_t)r * a.top_k + n] = logprob(x);
         ++n;
       }
   }
 }
 
-// d_logits = g ([i == target] - p_i) - h p_i (log p_i + H); pieces of a row, kPieces per thread
+// d_logits = g ([i == target] - p_i) - h p_i (log p_i + H); pieces of a row, kPieces per thread.  4096 x 50288 bf16 with the
+// entropy's gradient: 151 us with five CTAs an SM, 161 with six (spills), 166 with four; fp32 255 us with six, 275 with five.
 constexpr int kBwdThreads = 256, kPieces = 4;
 template <typename T, bool kEntropy>
-__global__ void __launch_bounds__(kBwdThreads, 6) logprobs_bwd_kernel(const __grid_constant__ qb_logprobs_args a, int parts) {
+__global__ void __launch_bounds__(kBwdThreads, sizeof(T) == 2 ? 5 : 6) logprobs_bwd_kernel(const __grid_constant__ qb_logprobs_args a, int parts) {
   constexpr int kN = Wide<T>::kN;
-  const int64_t r = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x % parts);
-  const T* row = static_cast<const T*>(a.logits) + r / a.inner_rows * a.outer_stride + r % a.inner_rows * a.row_stride;
-  T* out = static_cast<T*>(a.d_logits) + r / a.inner_rows * a.d_outer_stride + r % a.inner_rows * a.d_row_stride;
+  const uint32_t r = blockIdx.x / (uint32_t)parts;
+  const int part = (int)(blockIdx.x % (uint32_t)parts);
+  const T* row = static_cast<const T*>(a.logits) + row_at(a, r, a.outer_stride, a.row_stride);
+  T* out = static_cast<T*>(a.d_logits) + row_at(a, r, a.d_outer_stride, a.d_row_stride);
   const int64_t t = a.targets[r];
   const bool kept = t != a.ignore_index && t >= 0 && t < a.vocab;
   const int target = kept ? (int)t : -1;
@@ -380,18 +442,21 @@ __global__ void __launch_bounds__(kBwdThreads, 6) logprobs_bwd_kernel(const __gr
   const uintptr_t ai = reinterpret_cast<uintptr_t>(row) & 15, ao = reinterpret_cast<uintptr_t>(out) & 15;
   const int head = ai == ao ? min(a.vocab, (int)((16 - ai) & 15) / (int)sizeof(T)) : a.vocab;   // not alike: one by one
   const int body = (a.vocab - head) / kN;
+  // a CTA's share of the pieces: all that its threads take at once, or (fp32, 255 us against 268) as many as the others
   constexpr int kStep = kBwdThreads * kPieces;
-  for (int i0 = part * kStep; i0 < body; i0 += parts * kStep) {
+  const int share = sizeof(T) == 2 ? kStep : (body / parts / kBwdThreads + 1) * kBwdThreads;
+  const int from = part * share, to = min(body, from + share);
+  for (int i0 = from; i0 < to; i0 += kStep) {
     Wide<T> v[kPieces];
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
       const int i = i0 + k * kBwdThreads + (int)threadIdx.x;
-      if (i < body) v[k] = load16(row + head + i * kN);
+      if (i < to) v[k] = load16(row + head + i * kN);
     }
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
       const int i = i0 + k * kBwdThreads + (int)threadIdx.x, c = head + i * kN;
-      if (i >= body) break;
+      if (i >= to) break;
       float d[kN];
 #pragma unroll
       for (int j = 0; j < kN; j += 2) unpack2(two(val(v[k].v[j]), val(v[k].v[j + 1])), d[j], d[j + 1]);
@@ -425,7 +490,7 @@ int check_logprobs(const qb_logprobs_args* a, const char* who) {
 template <typename T, int kThreads, bool kEntropy, bool kAlt>
 int launch_logprobs(const qb_logprobs_args& a, int* status, cudaStream_t st) {
   // CTAs of a row: as many in all as are resident at once, with a piece per thread at least
-  constexpr int kResident = kAlt && kThreads == 512 ? 2 : 2048 / kThreads;
+  constexpr int kResident = kThreads == 64 ? 32 : kAlt ? 2 : 6;
   int64_t parts = 1;
   while (parts < kMaxCluster && a.rows * parts * 2 <= (int64_t)sm_count() * kResident && a.vocab / (parts * 2) >= kThreads * Wide<T>::kN) parts *= 2;
   const int64_t unit = 128 / (int64_t)sizeof(T), part_len = ceil_div(ceil_div(a.vocab, parts), unit) * unit;

@@ -96,6 +96,17 @@ def test_slices_of_a_batch(dtype):
 
 
 @pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("rows", [1, 700])
+def test_numbers_come_before_nan_on_a_plateau(rows, dtype):
+    """More equal values than a part lists, one NaN among them: the lowest columns with a number, whatever the row's parts."""
+    logits = torch.ones(rows, 50280, dtype=dtype, device="cuda")
+    logits[:, 3] = float("nan")
+    r, _ = run(logits, torch.zeros(rows, dtype=torch.int64, device="cuda"), 5)
+    assert torch.equal(r.top_ids, torch.tensor([0, 1, 2, 4, 5], device="cuda").expand(rows, -1))
+    assert r.top_logprobs.isnan().all() and r.logprobs.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("top_k", [1, 9, 32])
 def test_ties_go_to_the_lowest_column(top_k, dtype):
     g = torch.Generator().manual_seed(4)
