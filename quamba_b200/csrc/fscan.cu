@@ -144,10 +144,7 @@ __device__ __forceinline__ void load_pairs(const float* p, f2 (&v)[kPairs]) {
 }
 template <int kCh>
 __device__ __forceinline__ void load_channels(const float* p, float (&v)[kCh]) {
-  if constexpr (kCh == 4) {
-    const float4 w = *reinterpret_cast<const float4*>(p);
-    v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-  } else if constexpr (kCh == 2) {
+  if constexpr (kCh == 2) {
     const float2 w = *reinterpret_cast<const float2*>(p);
     v[0] = w.x; v[1] = w.y;
   } else {
@@ -170,69 +167,29 @@ __device__ __forceinline__ float own_channel(const float (&v)[kCh], int q) {
   return a;
 }
 
-// Sums over the lanes of one q of kNp values each, four tokens at a time.  Sixteen values a lane go through shared memory: a lane leaves
-// them as 16-byte pieces, then every lane adds up an output piece (t, n .. n + 3) over the groups (2 x 1024 tokens of 5120 channels of 64
-// states: 1.76 ms, 2.44 by shuffles).  Eight go by shuffles that halve the list at every step: there the way through
-// shared memory takes fewer instructions but more time (1.15 ms for 8 x 1024 tokens of 5120 channels of 16 states, 1.10 by shuffles).
-template <typename G, bool kShared = G::kNp == 16>
-struct GroupSums {
-  static constexpr int kTokens = 4, kRow = 32 * G::kNp + 16, kPer = G::kNp / 4;
-  float v[kTokens][kRow];
-  static __device__ __forceinline__ int place(int lane, int piece) { return lane * G::kNp + (piece ^ (kPer == 2 ? (lane >> 2) & 1 : (lane >> 1) & 3)) * 4; }
-  __device__ __forceinline__ void put(int t, int lane, const f2 (&s)[G::kPairs], float*) {
-#pragma unroll
-    for (int p = 0; p < kPer; ++p) *reinterpret_cast<ulonglong2*>(&v[t][place(lane, p)]) = make_ulonglong2(s[2 * p], s[2 * p + 1]);
-  }
-  // out: [4][out_row] with the kN sums of a token first
-  __device__ __forceinline__ void take(int lane, float* out, int out_row) const {
-    __syncwarp();
-    constexpr int kPieces = kTokens * G::kN / 4, kShare = kPieces < 32 ? 32 / kPieces : 1, kGroups = 32 / G::kQ / kShare;
-#pragma unroll
-    for (int i = lane / kShare; i < kPieces; i += 32 / kShare) {
-      const int t = i / (G::kN / 4), n4 = i % (G::kN / 4), q = n4 / kPer, piece = n4 % kPer, g0 = lane % kShare * kGroups;
-      f2 a = 0ull, b = 0ull;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&v[t][place((g0 + g) * G::kQ + q, piece)]);
-        a = g == 0 ? w.x : add2(a, w.x);
-        b = g == 0 ? w.y : add2(b, w.y);
-      }
-      float x[4];
-      unpack2(a, x[0], x[1]);
-      unpack2(b, x[2], x[3]);
-      if (kShare == 2)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] += __shfl_xor_sync(0xffffffffu, x[k], 1);
-      if (lane % kShare == 0) *reinterpret_cast<float4*>(out + t * out_row + n4 * 4) = make_float4(x[0], x[1], x[2], x[3]);
-    }
-    __syncwarp();
-  }
-};
+// A token's sums, over the lanes of one q, of kNp values each go to out: shuffles that halve the list at every step.  (Through shared
+// memory they take fewer instructions but more time: 1.15 ms for 8 x 1024 tokens of 5120 channels of 16 states, 1.10 by shuffles.)
 template <typename G>
-struct GroupSums<G, false> {
-  // the token's sums of this lane's q go to out
-  __device__ __forceinline__ void put(int, int lane, const f2 (&s)[G::kPairs], float* out) {
-    float v[G::kNp];
+__device__ __forceinline__ void group_sums(int lane, const f2 (&s)[G::kPairs], float* out) {
+  float v[G::kNp];
 #pragma unroll
-    for (int p = 0; p < G::kPairs; ++p) unpack2(s[p], v[2 * p], v[2 * p + 1]);
-    int at = 0, left = G::kNp;
+  for (int p = 0; p < G::kPairs; ++p) unpack2(s[p], v[2 * p], v[2 * p + 1]);
+  int at = 0, left = G::kNp;
 #pragma unroll
-    for (int bit = 16; bit >= G::kQ; bit >>= 1) {
-      const bool up = lane & bit;
-      if (left > 1) {
-        left /= 2;
+  for (int bit = 16; bit >= G::kQ; bit >>= 1) {
+    const bool up = lane & bit;
+    if (left > 1) {
+      left /= 2;
 #pragma unroll
-        for (int k = 0; k < left; ++k) v[k] = (up ? v[left + k] : v[k]) + __shfl_xor_sync(0xffffffffu, up ? v[k] : v[left + k], bit);
-        at += up ? left : 0;
-      } else {
-        v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);     // both hold the sum
-      }
+      for (int k = 0; k < left; ++k) v[k] = (up ? v[left + k] : v[k]) + __shfl_xor_sync(0xffffffffu, up ? v[k] : v[left + k], bit);
+      at += up ? left : 0;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);       // both hold the sum
     }
-#pragma unroll
-    for (int k = 0; k < left; ++k) out[at + k] = v[k];
   }
-  __device__ __forceinline__ void take(int, float*, int) const {}
-};
+#pragma unroll
+  for (int k = 0; k < left; ++k) out[at + k] = v[k];
+}
 
 // a token's decays, and its step of the states
 template <typename G>
@@ -687,7 +644,6 @@ struct alignas(16) BwdWarpSmem {            // one behind the other for the CTA'
   float inner[kT][G::kWc], through[kT][G::kWc], into[kT][G::kWc];
   float bc[2][kT][G::kN];
   float part[kT][2][G::kN];
-  GroupSums<G> sums;
 };
 
 // a lane's 8 or 16 floats to and from its row of tensor memory
@@ -742,10 +698,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks<G>)
 float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nseg, int seg_len, const float* sums, float* part_bc, float* part_grad,
                       Vec vec) {
   using S = BwdWarpSmem<T, G>;
-  static_assert(sizeof(S) % 16 == 0 && offsetof(S, delta) % 16 == 0 && offsetof(S, bc) % 16 == 0 && offsetof(S, part) % 16 == 0 && offsetof(S, sums) % 16 == 0,
+  static_assert(sizeof(S) % 16 == 0 && offsetof(S, delta) % 16 == 0 && offsetof(S, bc) % 16 == 0 && offsetof(S, part) % 16 == 0,
                 "16-byte accesses");
   constexpr int kT = S::kT, kBuf = S::kBuf, kNp = G::kNp, kStates = G::kCh * kNp, kColumns = kT * kStates;
-  constexpr int kTurn = G::kNp == 16 ? 4 : kT;           // tokens between two GroupSums::take
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ uint32_t s_tmem;
   const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
@@ -861,95 +816,87 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
     widen_bc<T, G, kT>(raw, s.bc, t0, lim, a.dstate, lane);
     __syncwarp();
     // forward: C . h, and dC's sums over the warp's channels
-#pragma unroll 1
-    for (int turn = 0; turn < kT; turn += kTurn) {
 #pragma unroll 2
-      for (int t = turn; t < turn + kTurn; ++t) {
-        float d[G::kCh], u[G::kCh], g[G::kCh], y[G::kCh];
-        f2 b2[G::kPairs], c2[G::kPairs], sC[G::kPairs], acc[G::kCh], e[G::kCh][G::kPairs];
-        load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
-        decays<G>(d, A, e);
-        load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
-        load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
-        load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
-        load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
-        tmem_keep<G>(tmem + t * kStates, h);
-        advance<G>(e, u, b2, h);
+    for (int t = 0; t < kT; ++t) {
+      float d[G::kCh], u[G::kCh], g[G::kCh], y[G::kCh];
+      f2 b2[G::kPairs], c2[G::kPairs], sC[G::kPairs], acc[G::kCh], e[G::kCh][G::kPairs];
+      load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
+      decays<G>(d, A, e);
+      load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
+      load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
+      load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
+      load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
+      tmem_keep<G>(tmem + t * kStates, h);
+      advance<G>(e, u, b2, h);
 #pragma unroll
-        for (int p = 0; p < G::kPairs; ++p)
-#pragma unroll
-          for (int c = 0; c < G::kCh; ++c) {
-            acc[c] = p == 0 ? mul2(h[c][0], c2[0]) : fma2(h[c][p], c2[p], acc[c]);
-            sC[p] = c == 0 ? mul2(pack2(g[0], g[0]), h[0][p]) : fma2(pack2(g[c], g[c]), h[c][p], sC[p]);
-          }
+      for (int p = 0; p < G::kPairs; ++p)
 #pragma unroll
         for (int c = 0; c < G::kCh; ++c) {
-          float lo, hi;
-          unpack2(acc[c], lo, hi);
-          y[c] = lo + hi;
+          acc[c] = p == 0 ? mul2(h[c][0], c2[0]) : fma2(h[c][p], c2[p], acc[c]);
+          sC[p] = c == 0 ? mul2(pack2(g[0], g[0]), h[0][p]) : fma2(pack2(g[c], g[c]), h[c][p], sC[p]);
         }
-        const float own = own_channel<G::kCh, G::kQ>(y, w.q);
-        if (w.q % (G::kQ / G::kCh) == 0) s.inner[t][w.own] = own;
-        s.sums.put(t % 4, lane, sC, &s.part[t][1][w.q * kNp]);
+#pragma unroll
+      for (int c = 0; c < G::kCh; ++c) {
+        float lo, hi;
+        unpack2(acc[c], lo, hi);
+        y[c] = lo + hi;
       }
-      s.sums.take(lane, &s.part[turn][1][0], 2 * G::kN);
+      const float own = own_channel<G::kCh, G::kQ>(y, w.q);
+      if (w.q % (G::kQ / G::kCh) == 0) s.inner[t][w.own] = own;
+      group_sums<G>(lane, sC, &s.part[t][1][w.q * kNp]);
     }
     tmem_kept_wait();
     // and back
-#pragma unroll 1
-    for (int turn = kT - kTurn; turn >= 0; turn -= kTurn) {
 #pragma unroll 2
-      for (int t = turn + kTurn - 1; t >= turn; --t) {
-        float d[G::kCh], u[G::kCh], g[G::kCh], through[G::kCh], into[G::kCh];
-        f2 b2[G::kPairs], c2[G::kPairs], sB[G::kPairs], e[G::kCh][G::kPairs], dh[G::kCh][G::kPairs], thr[G::kCh], q2[G::kCh];
-        uint32_t kept[16];
-        tmem_fetch<G>(tmem + t * kStates, kept);
-        load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
-        decays<G>(d, A, e);
-        load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
-        load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
-        load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
-        load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
+    for (int t = kT - 1; t >= 0; --t) {
+      float d[G::kCh], u[G::kCh], g[G::kCh], through[G::kCh], into[G::kCh];
+      f2 b2[G::kPairs], c2[G::kPairs], sB[G::kPairs], e[G::kCh][G::kPairs], dh[G::kCh][G::kPairs], thr[G::kCh], q2[G::kCh];
+      uint32_t kept[16];
+      tmem_fetch<G>(tmem + t * kStates, kept);
+      load_channels<G::kCh>(&s.delta[t][w.cg * G::kCh], d);
+      decays<G>(d, A, e);
+      load_channels<G::kCh>(&s.u[t][w.cg * G::kCh], u);
+      load_channels<G::kCh>(&s.g[t][w.cg * G::kCh], g);
+      load_pairs<G::kPairs>(&s.bc[0][t][w.q * kNp], b2);
+      load_pairs<G::kPairs>(&s.bc[1][t][w.q * kNp], c2);
 #pragma unroll
-        for (int c = 0; c < G::kCh; ++c)
+      for (int c = 0; c < G::kCh; ++c)
 #pragma unroll
-          for (int p = 0; p < G::kPairs; ++p) dh[c][p] = fma2(c2[p], pack2(g[c], g[c]), carry[c][p]);
+        for (int p = 0; p < G::kPairs; ++p) dh[c][p] = fma2(c2[p], pack2(g[c], g[c]), carry[c][p]);
 #pragma unroll
-        for (int c = 0; c < G::kCh; ++c)
+      for (int c = 0; c < G::kCh; ++c)
 #pragma unroll
-          for (int p = 0; p < G::kPairs; ++p) carry[c][p] = mul2(dh[c][p], e[c][p]);
+        for (int p = 0; p < G::kPairs; ++p) carry[c][p] = mul2(dh[c][p], e[c][p]);
 #pragma unroll
-        for (int p = 0; p < G::kPairs; ++p)
-#pragma unroll
-          for (int c = 0; c < G::kCh; ++c) {
-            sB[p] = c == 0 ? mul2(pack2(u[0], u[0]), dh[0][p]) : fma2(pack2(u[c], u[c]), dh[c][p], sB[p]);
-            thr[c] = p == 0 ? mul2(dh[c][0], b2[0]) : fma2(dh[c][p], b2[p], thr[c]);
-          }
-        tmem_fetched<G>(kept, h);
-#pragma unroll
-        for (int p = 0; p < G::kPairs; ++p)
-#pragma unroll
-          for (int c = 0; c < G::kCh; ++c) {
-            dh[c][p] = mul2(carry[c][p], h[c][p]);
-            q2[c] = p == 0 ? mul2(dh[c][0], A[c][0]) : fma2(dh[c][p], A[c][p], q2[c]);
-            dA[c][p] = fma2(dh[c][p], pack2(d[c], d[c]), dA[c][p]);
-          }
+      for (int p = 0; p < G::kPairs; ++p)
 #pragma unroll
         for (int c = 0; c < G::kCh; ++c) {
-          float lo, hi;
-          unpack2(thr[c], lo, hi);
-          through[c] = lo + hi;
-          unpack2(q2[c], lo, hi);
-          into[c] = lo + hi;
+          sB[p] = c == 0 ? mul2(pack2(u[0], u[0]), dh[0][p]) : fma2(pack2(u[c], u[c]), dh[c][p], sB[p]);
+          thr[c] = p == 0 ? mul2(dh[c][0], b2[0]) : fma2(dh[c][p], b2[p], thr[c]);
         }
-        s.sums.put(t % 4, lane, sB, &s.part[t][0][w.q * kNp]);
-        const float own_through = own_channel<G::kCh, G::kQ>(through, w.q), own_into = own_channel<G::kCh, G::kQ>(into, w.q);
-        if (w.q % (G::kQ / G::kCh) == 0) {
-          s.through[t][w.own] = own_through;
-          s.into[t][w.own] = own_into;
+      tmem_fetched<G>(kept, h);
+#pragma unroll
+      for (int p = 0; p < G::kPairs; ++p)
+#pragma unroll
+        for (int c = 0; c < G::kCh; ++c) {
+          dh[c][p] = mul2(carry[c][p], h[c][p]);
+          q2[c] = p == 0 ? mul2(dh[c][0], A[c][0]) : fma2(dh[c][p], A[c][p], q2[c]);
+          dA[c][p] = fma2(dh[c][p], pack2(d[c], d[c]), dA[c][p]);
         }
+#pragma unroll
+      for (int c = 0; c < G::kCh; ++c) {
+        float lo, hi;
+        unpack2(thr[c], lo, hi);
+        through[c] = lo + hi;
+        unpack2(q2[c], lo, hi);
+        into[c] = lo + hi;
       }
-      s.sums.take(lane, &s.part[turn][0][0], 2 * G::kN);
+      group_sums<G>(lane, sB, &s.part[t][0][w.q * kNp]);
+      const float own_through = own_channel<G::kCh, G::kQ>(through, w.q), own_into = own_channel<G::kCh, G::kQ>(into, w.q);
+      if (w.q % (G::kQ / G::kCh) == 0) {
+        s.through[t][w.own] = own_through;
+        s.into[t][w.own] = own_into;
+      }
     }
     if (chunk % 2 == 1) {                                // the middle of a tile of the forward pass
       float two[G::kCh], more[G::kCh];
@@ -1197,11 +1144,12 @@ void cut(Plan& p, int seqlen, int64_t want) {
   p.nseg = (int)std::max<int64_t>(1, ceil_div(seqlen, p.seg_len));
 }
 // Forward.  Eight states a lane: sixteen take fewer instructions but leave too few warps on an SM to hide each one's latencies
-// (8 x 1024 tokens of 5120 channels: 389 us against 440).  Rows that put fewer than eight warps on an SM are cut into segments, which are
-// walked twice (512 tokens of 1536 channels: 28 us, in one piece 68; 4 x 2048 of 5120, nine warps: 515, cut in four 532).  A
+// (8 x 1024 tokens of 5120 channels: 374 us against 440).  More than 32 states: eight of two channels, as on the way back (2 x 1024 tokens of
+// 5120 channels: 409 us, sixteen of one channel 511, eight of one 689).  Rows that put fewer than eight warps on an SM are cut into segments, which are
+// walked twice (512 tokens of 1536 channels: 27 us, in one piece 68; 4 x 2048 of 5120, nine warps: 488, cut in four 532).  A
 // short sequence cannot be cut often enough and takes four states a lane.
 Plan plan_fwd(int batch, int seqlen, int dim, int groups, int dstate) {
-  Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 1, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 1, 4) : share_of(batch, dim, groups, 16, 1, 4);
+  Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 1, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 1, 4) : share_of(batch, dim, groups, 8, 2, 8);
   const int64_t sms = sm_count();
   if (dstate <= 16 && (int64_t)batch * p.tiles < 8 * sms && (int64_t)batch * p.tiles * std::max(1, seqlen / kMinSeg) < 12 * sms)
     p = share_of(batch, dim, groups, 4, 1, 4);
@@ -1209,17 +1157,20 @@ Plan plan_fwd(int batch, int seqlen, int dim, int groups, int dstate) {
   cut(p, seqlen, warps >= 8 * sms ? 1 : ceil_div(32 * sms, warps));
   return p;
 }
-// Backward: sixteen states a lane where that gives every SM four warps, else eight; and as many segments as make the number of
-// waves of resident CTAs (four an SM) times a segment's length smallest.  A segment's summary costs a quarter of its walk.  8 x 1024
-// tokens of 5120 channels: 1.26 ms in twelve segments, 1.54 in one piece.
+// Backward: sixteen states a lane, in as many segments as make the number of waves of resident CTAs (three an SM) times a segment's
+// length smallest.  A segment's summary costs a quarter of its walk.  8 x 1024 tokens of 5120 channels: 1.08 ms, in one piece 1.54;
+// 16384 of 2048 fp32: 0.93 ms in 27 segments, 1.05 in 24, 1.13 with eight states a lane.  Where even the most segments leave an SM fewer
+// than six warps, eight a lane (4 x 256 tokens of 1536 channels: 79 us against 89; 16 x 64 of 2048, seven warps: 77 against 69).
+// Up to 64 states lie on eight lanes of two channels (2 x 1024 tokens of 5120 channels: 1.13 ms; sixteen a lane of one channel, with twice
+// the reads of B and C: 1.76).
 Plan plan_bwd(int batch, int seqlen, int dim, int groups, int dstate) {
   const int64_t sms = sm_count();
-  Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 2, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 2, 4) : share_of(batch, dim, groups, 16, 1, 4);
-  if (p.ch == 2 && (int64_t)batch * p.tiles < 4 * sms) p = share_of(batch, dim, groups, 8, 1, p.q);
-  const int64_t ctas = std::max<int64_t>(1, (int64_t)batch * groups * ceil_div(p.tpg, kBwdWarps)), slots = (p.np == 16 ? 2 : p.ch == 2 ? 3 : 4) * sms;
+  Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 2, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 2, 4) : share_of(batch, dim, groups, 8, 2, 8);
+  if (dstate <= 32 && (int64_t)batch * p.tiles * std::min(kMaxSegs, std::max(1, seqlen / kMinSeg)) < 6 * sms) p = share_of(batch, dim, groups, 8, 1, p.q);
+  const int64_t ctas = std::max<int64_t>(1, (int64_t)batch * groups * ceil_div(p.tpg, kBwdWarps)), slots = (p.ch == 2 ? 3 : 4) * sms;
   int64_t best = 1;
   double least = 0.0;
-  for (int64_t n = 1; n <= std::min<int64_t>(24, std::max(1, seqlen / kMinSeg)); ++n) {
+  for (int64_t n = 1; n <= std::min<int64_t>(kMaxSegs, std::max(1, seqlen / kMinSeg)); ++n) {
     const double cost = (double)ceil_div(ctas * n, slots) / n * (1.0 + 0.25 * (n - 1) / n);
     if (n == 1 || cost < least) { least = cost; best = n; }
   }
@@ -1329,14 +1280,12 @@ int by_type(int dtype, F f) {
 template <typename F>
 int by_share_fwd(const Plan& p, F f) {
   if (p.np == 4) return f(Geo<4, 1, 4>{});
-  if (p.np == 8) return p.q == 2 ? f(Geo<8, 1, 2>{}) : f(Geo<8, 1, 4>{});
-  return f(Geo<16, 1, 4>{});
+  return p.q == 2 ? f(Geo<8, 1, 2>{}) : p.q == 4 ? f(Geo<8, 1, 4>{}) : f(Geo<8, 2, 8>{});
 }
 template <typename F>
 int by_share_bwd(const Plan& p, F f) {
-  if (p.q == 2) return p.ch == 2 ? f(Geo<8, 2, 2>{}) : f(Geo<8, 1, 2>{});
-  if (p.np == 8) return p.ch == 2 ? f(Geo<8, 2, 4>{}) : f(Geo<8, 1, 4>{});
-  return f(Geo<16, 1, 4>{});
+  if (p.ch == 1) return p.q == 2 ? f(Geo<8, 1, 2>{}) : f(Geo<8, 1, 4>{});
+  return p.q == 2 ? f(Geo<8, 2, 2>{}) : p.q == 4 ? f(Geo<8, 2, 4>{}) : f(Geo<8, 2, 8>{});
 }
 
 }  // namespace
