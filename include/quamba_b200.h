@@ -806,7 +806,7 @@ int qb_sum_partials(const void* partials, int32_t n_partials, int64_t partial_st
  * one type (dtype 0 float32, 1 float16, 2 bfloat16), unit stride in the last dim.  A (dim, dstate), D, dt_bias (dim),
  * initial_state, final_state (batch, dim, dstate): float32, contiguous; D, dt_bias, z, initial_state, final_state may be
  * NULL.  lengths (batch) int32 on the device, or NULL: tokens from lengths[b] on are not part of sequence b -- what lies
- * there is not used, y and every gradient is 0 there; values outside 0..seqlen count as the nearer end.  1 <= dstate <= 64.
+ * there is not used, y and every gradient is 0 there; values outside 0..seqlen count as the nearer end.  1 <= dstate <= 64, seqlen <= 2^30.
  * y and the gradients of x, dt, z, B, C are contiguous.
  *
  * qb_float_scan_fwd: y and final_state; with checkpoints != NULL also the states every 8 tokens, in the library's own
@@ -909,7 +909,7 @@ int qb_float_scan_update(const qb_float_update_args* a, void* stream);
  *   lse        = log sum_i exp(x_i)                              logprobs[r] = x_target - lse
  *   entropy[r] = lse - sum_i p_i x_i, p_i = exp(x_i - lse)       (entropy may be NULL)
  *   top_logprobs / top_ids (rows, top_k): the top_k largest logits' log probabilities and columns, largest first, equal
- *   values in the order of their columns; 0 <= top_k <= 32, top_k <= vocab.
+ *   values in the order of their columns; 0 <= top_k <= 32, top_k <= vocab <= 2^30.
  * A column of -inf has probability 0.  A row of nothing but -inf has no distribution: log probabilities -inf, entropy 0 and
  * gradient 0.  A row that holds a NaN or +inf gives NaN (and some columns of the row as top_ids).  targets int64 (rows): ignore_index
  * gives logprobs 0 without gradient; any other value outside 0..vocab-1 gives NaN and sets the device status word.

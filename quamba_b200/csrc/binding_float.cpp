@@ -67,7 +67,7 @@ struct ScanIn {
       lengths = contiguous(lengths);
     }
     softplus = a.flag(8);
-    need(std::max({batch, len, dim}) < (1ll << 31), "the tensors are too large");
+    need(std::max(batch, dim) < (1ll << 31) && len <= (1ll << 30), "the tensors are too large");
   }
   qb_float_scan_args args() const {
     qb_float_scan_args s{};
@@ -81,6 +81,30 @@ struct ScanIn {
     return s;
   }
 };
+
+// Whether float32 tensors of n consecutive values a row are the same rows or share none (rows that interleave some other way than
+// with equal strides count as shared).
+bool same_or_apart(const Tensor& a, const Tensor& b, int64_t n) {
+  if (a.numel() == 0) return true;
+  std::vector<int64_t> steps;
+  int64_t reach_a = n, reach_b = n;
+  bool alike = true;
+  for (int i = 0; i < 2; ++i) {
+    if (a.size(i) == 1) continue;
+    alike = alike && a.stride(i) == b.stride(i);
+    reach_a += (a.size(i) - 1) * a.stride(i);
+    reach_b += (b.size(i) - 1) * b.stride(i);
+    steps.push_back(a.stride(i));
+  }
+  const float *pa = static_cast<const float*>(a.data_ptr()), *pb = static_cast<const float*>(b.data_ptr());
+  if (pa + reach_a <= pb || pb + reach_b <= pa || (alike && pa == pb)) return true;
+  if (!alike || steps.empty()) return false;
+  std::sort(steps.begin(), steps.end());
+  const int64_t small = steps.front(), big = steps.back(), off = std::abs(pb - pa) % big;
+  for (const int64_t r : {off, big - off})
+    if (r % small < n || small - r % small < n) return false;
+  return true;
+}
 
 // A workspace or the kept states; the stand-in for an empty tensor's address (which may be null) is never read.
 Tensor bytes_of(const Device& dev, int64_t bytes) { return dev.empty({std::max<int64_t>(bytes, 16)}, at::kByte); }
@@ -120,7 +144,7 @@ PyObject* float_scan_bwd(const Args& a) {
   Device dev(in.x);
   const auto type = in.x.scalar_type();
   Tensor dx = dev.empty({in.batch, in.len, in.dim}, type), ddt = dev.empty({in.batch, in.len, in.dim}, type), dA = dev.empty({in.dim, in.n}, at::kFloat);
-  Tensor dB = dev.empty({in.batch, in.len, in.groups, in.n}, type), dC = dev.empty({in.batch, in.len, in.groups, in.n}, type);
+  Tensor dB = dev.empty(a.tensor(3).sizes(), type), dC = dev.empty(a.tensor(4).sizes(), type);     // with or without groups, as they came
   Tensor dD, dz, dbias, dinit;
   if (in.D.defined()) dD = dev.empty({in.dim}, at::kFloat);
   if (in.z.defined()) dz = dev.empty({in.batch, in.len, in.dim}, type);
@@ -165,6 +189,7 @@ PyObject* float_scan_update(const Args& a) {
   need(batch * dim == 0 || ((batch == 1 || so.stride(0) >= n) && (dim == 1 || so.stride(1) >= n) &&
                             (batch == 1 || dim == 1 || so.stride(0) >= (dim - 1) * so.stride(1) + n || so.stride(1) >= (batch - 1) * so.stride(0) + n)),
        "the rows of state_out must not overlap");
+  need(same_or_apart(st, so, n), "state_out must be state itself or share no memory with it");
   for (Tensor* t : {&B, &C}) {
     const char* name = t == &B ? "B" : "C";
     need(t->dim() == 2 || t->dim() == 3, said(name, " must be (batch, dstate) or (batch, groups, dstate)"));
@@ -203,7 +228,7 @@ struct LogitsIn {
     code = type_code(l, "logits");
     need(l.dim() == 2 || l.dim() == 3, "logits must be (rows, vocab) or (batch, seqlen, vocab)");
     vocab = l.size(-1);
-    need(vocab > 0 && vocab < (1ll << 31), "logits must have a vocabulary of 1 to 2^31 - 1 columns");
+    need(vocab > 0 && vocab <= (1ll << 30), "logits must have a vocabulary of 1 to 2^30 columns");
     need(vocab == 1 || l.stride(-1) == 1, "logits must be contiguous in their last dim");
     need(t.is_cuda() && t.device() == l.device() && t.scalar_type() == at::kLong, "targets must be an int64 CUDA tensor on the logits' device");
     need(t.sizes() == l.sizes().slice(0, l.dim() - 1), "targets must have the shape of the logits without the vocabulary");

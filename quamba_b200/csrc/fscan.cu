@@ -1197,6 +1197,7 @@ int check_scan(const qb_float_scan_args* a, bool backward) {
   QB_REQUIRE(a != nullptr && a->x && a->dt && a->Bm && a->Cm && a->A, QB_ERR_INVALID_ARG, "%s: null pointer", who);
   QB_REQUIRE(a->dstate >= 1 && a->dstate <= 64, QB_ERR_INVALID_ARG, "%s: dstate must be 1 to 64, got %d", who, a->dstate);
   QB_REQUIRE(a->batch >= 0 && a->seqlen >= 0 && a->dim > 0 && a->groups > 0, QB_ERR_INVALID_ARG, "%s: bad shape", who);
+  QB_REQUIRE(a->seqlen <= 1 << 30, QB_ERR_TOO_LARGE, "%s: more than 2^30 tokens in a sequence", who);   // a tile or segment more still fits an int
   QB_REQUIRE(a->dim % a->groups == 0, QB_ERR_INVALID_ARG, "%s: dim = %d is not divisible by groups = %d", who, a->dim, a->groups);
   QB_REQUIRE(a->dtype >= 0 && a->dtype <= 2, QB_ERR_INVALID_ARG, "%s: unsupported type", who);
   const Plan p = plan_of(a->batch, a->seqlen, a->dim, a->groups, a->dstate, backward);
@@ -1348,7 +1349,7 @@ extern "C" int qb_float_scan_update(const qb_float_update_args* a, void* stream)
   // sequences of a thread: as many as leave every SM six CTAs, in whole turns of kAhead (64 x 5120 x 16 states: 17 us, one each 37)
   const int64_t share = std::max<int64_t>(1, std::min<int64_t>(a->batch, ceil_div(across * a->batch, 6 * sm_count())));
   const int64_t rows = share > 2 ? ceil_div(share, kAhead) * kAhead : share, down = ceil_div(a->batch, rows);
-  QB_REQUIRE(across < (1ll << 31) && down < 65536, QB_ERR_TOO_LARGE, "float_scan_update: batch and dim are too large");
+  QB_REQUIRE(across < (1ll << 24) && down < 65536, QB_ERR_TOO_LARGE, "float_scan_update: batch and dim are too large");
   const size_t size = a->dtype == 0 ? 4 : 2;
   const int vec = a->dstate % 4 == 0 && aligned(a->state, 16) && aligned(a->state_out, 16) &&
                   (a->state_sb | a->state_sd | a->state_out_sb | a->state_out_sd) % 4 == 0;

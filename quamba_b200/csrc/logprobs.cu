@@ -481,6 +481,7 @@ __global__ void __launch_bounds__(kBwdThreads, sizeof(T) == 2 ? 5 : 6) logprobs_
 int check_logprobs(const qb_logprobs_args* a, const char* who) {
   QB_REQUIRE(a != nullptr, QB_ERR_INVALID_ARG, "%s: null pointer", who);
   QB_REQUIRE(a->rows >= 0 && a->vocab > 0 && (a->rows == 0 || a->inner_rows > 0), QB_ERR_INVALID_ARG, "%s: bad shape", who);
+  QB_REQUIRE(a->vocab <= 1 << 30, QB_ERR_TOO_LARGE, "%s: more than 2^30 columns", who);        // a part more still fits an int
   QB_REQUIRE(a->dtype >= 0 && a->dtype <= 2, QB_ERR_INVALID_ARG, "%s: unsupported type", who);
   QB_REQUIRE(a->rows == 0 || (a->logits != nullptr && a->targets != nullptr), QB_ERR_INVALID_ARG, "%s: null pointer", who);
   QB_REQUIRE(aligned(a->logits, a->dtype == 0 ? 4 : 2), QB_ERR_INVALID_ARG, "%s: logits are not aligned to their type", who);

@@ -38,7 +38,7 @@ class _SelectiveScan(torch.autograd.Function):
             dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
         dx, ddt, dA, dB, dC, dD, dz, dbias, dinit = _n().float_scan_bwd(x, dt, A, B, C, D, z, dt_bias, ctx.dt_softplus, initial_state, lengths, kept,
                                                                         dy, dlast)
-        return dx, ddt, dA, dB.view(B.shape), dC.view(C.shape), dD, dz, dbias, None, dinit, None
+        return dx, ddt, dA, dB, dC, dD, dz, dbias, None, dinit, None
 
 
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, initial_state=None, lengths=None,
@@ -67,6 +67,6 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
 def selective_scan_update(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, state_out=None):
     """One token per sequence: x, dt, z (batch, dim), B, C (batch, dstate) or (batch, groups, dstate), state float32
     (batch, dim, dstate), contiguous in its last dim.  Returns y (batch, dim); the state is advanced in place, or written to
-    ``state_out`` when that is given (its rows must not overlap, nor those of ``state`` unless it is the same tensor).  Types and
+    ``state_out`` when that is given (``state`` itself or memory that it shares nothing with).  Types and
     parameters as in :func:`selective_scan`; not differentiable."""
     return _n().float_scan_update(state, x, dt, A, B, C, D, z, dt_bias, dt_softplus, state_out)

@@ -54,9 +54,9 @@ def token_logprobs(logits, targets, top_k=0, return_entropy=False, ignore_index=
 
 
 def next_token_targets(input_ids, lengths=None, ignore_index=-100):
-    """The targets (batch, seqlen - 1) of a batch of token ids: each position's next token, ``ignore_index`` where that is at or past
+    """The targets (batch, seqlen - 1), int64, of a batch of token ids: each position's next token, ``ignore_index`` where that is at or past
     ``lengths[b]``."""
-    targets = input_ids[:, 1:]
+    targets = input_ids[:, 1:].to(torch.int64)
     if lengths is None:
         return targets
     lengths = torch.as_tensor(lengths, device=input_ids.device)

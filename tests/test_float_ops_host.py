@@ -51,6 +51,26 @@ def test_scan_arguments(kw, words):
         assert words in lib.qb_last_error()
 
 
+def test_what_would_pass_an_int_is_too_large():
+    lib = _lib.lib()
+    p = _scan_args().x
+    for fn in (lib.qb_float_scan_fwd, lib.qb_float_scan_bwd):
+        assert fn(ctypes.byref(_scan_args(seqlen=(1 << 30) + 1)), None) == _lib.QB_ERR_TOO_LARGE
+    step = _lib.make("qb_float_update_args", state=p, state_out=p, x=p, dt=p, Bm=p, Cm=p, A=p, y=p, batch=1, dim=1 << 30, dstate=16, groups=1)
+    assert lib.qb_float_scan_update(ctypes.byref(step), None) == _lib.QB_ERR_TOO_LARGE
+    row = _lib.make("qb_logprobs_args", logits=1 << 20, targets=1 << 20, logprobs=1 << 20, rows=1, inner_rows=1, vocab=(1 << 30) + 1, row_stride=1 << 31)
+    for fn in (lib.qb_logprobs_fwd, lib.qb_logprobs_bwd):
+        assert fn(ctypes.byref(row), None) == _lib.QB_ERR_TOO_LARGE
+
+
+def test_next_token_targets():
+    from quamba_b200.scoring import next_token_targets
+    ids = torch.tensor([[5, 6, 7, 8], [9, 3, 2, 1]], dtype=torch.int32)
+    assert next_token_targets(ids).tolist() == [[6, 7, 8], [3, 2, 1]] and next_token_targets(ids).dtype == torch.int64
+    assert next_token_targets(ids, [3, 1]).tolist() == [[6, 7, -100], [-100, -100, -100]]
+    assert next_token_targets(ids[:, :1]).shape == (2, 0)
+
+
 def test_backward_needs_its_workspace_and_checkpoints():
     lib = _lib.lib()
     assert lib.qb_float_scan_bwd(ctypes.byref(_scan_args()), None) == _lib.QB_ERR_INVALID_ARG

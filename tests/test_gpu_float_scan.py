@@ -388,3 +388,22 @@ def test_update_refusals():
             selective_scan_update(bad, **args)
     with pytest.raises(RuntimeError, match="state_out must be"):
         selective_scan_update(st, **args, state_out=st[:1])
+    rows = torch.zeros(3, 40, 32, device="cuda")
+    flat = torch.zeros(2 * 40 * 16 + 8, device="cuda")
+    for a, b in [(rows[:2, :, :16], rows[1:, :, :16]), (rows[:2, :, :16], rows[:2, :, 8:24]),
+                 (flat[:1280].view(2, 40, 16), flat[8:].view(2, 40, 16)), (flat[:1280].view(2, 40, 16), flat[:1280].view(40, 2, 16).transpose(0, 1))]:
+        with pytest.raises(RuntimeError, match="share no memory"):
+            selective_scan_update(a, **args, state_out=b)
+
+
+def test_update_of_interleaved_states():
+    """The old and the new state as two halves of the same rows: nothing is shared."""
+    from quamba_b200 import selective_scan_update
+    c = make(torch.float16, 2, 1, 40, 16)
+    args = dict(**step_inputs(c, 0), A=c["A"], D=c["D"], dt_bias=c["dt_bias"])
+    rows = torch.zeros(2, 40, 32, device="cuda")
+    rows[..., :16] = c["initial_state"]
+    out = torch.empty_like(c["initial_state"])
+    want = selective_scan_update(c["initial_state"], **args, state_out=out)
+    assert torch.equal(selective_scan_update(rows[..., :16], **args, state_out=rows[..., 16:]), want)
+    assert torch.equal(rows[..., 16:], out) and torch.equal(rows[..., :16], c["initial_state"])
