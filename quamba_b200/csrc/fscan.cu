@@ -1129,7 +1129,7 @@ struct Plan {
   int rec() const { return 32 * np * ch; }
   int wide() const { return np * q; }
 };
-constexpr int kMinSeg = 64;                // tokens of a segment, at least
+constexpr int kMinSeg = 32;                // tokens of a segment, at least
 constexpr int kMaxSegs = 32;               // a segment folds the summaries of all on its one side
 
 Plan share_of(int batch, int dim, int groups, int np, int ch, int q) {
@@ -1146,8 +1146,9 @@ void cut(Plan& p, int seqlen, int64_t want) {
 // Forward.  Eight states a lane: sixteen take fewer instructions but leave too few warps on an SM to hide each one's latencies
 // (8 x 1024 tokens of 5120 channels: 374 us against 440).  More than 32 states: eight of two channels, as on the way back (2 x 1024 tokens of
 // 5120 channels: 409 us, sixteen of one channel 511, eight of one 689).  Rows that put fewer than eight warps on an SM are cut into segments, which are
-// walked twice (512 tokens of 1536 channels: 27 us, in one piece 68; 4 x 2048 of 5120, nine warps: 488, cut in four 532).  A
-// short sequence cannot be cut often enough and takes four states a lane.
+// walked twice (512 tokens of 1536 channels: 25 us, in one piece 68; 4 x 2048 of 5120, nine warps: 488, cut in four 532).  Pieces of 32
+// tokens are the shortest (2 x 333 tokens of 1536 channels: 28 us, of 64 34, of 16 27, but 4 x 256 33, 38 and 36).  What fewer than six warps
+// an SM are left of then takes four states a lane.
 Plan plan_fwd(int batch, int seqlen, int dim, int groups, int dstate) {
   Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 1, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 1, 4) : share_of(batch, dim, groups, 8, 2, 8);
   const int64_t sms = sm_count();
@@ -1158,19 +1159,21 @@ Plan plan_fwd(int batch, int seqlen, int dim, int groups, int dstate) {
   return p;
 }
 // Backward: sixteen states a lane, in as many segments as make the number of waves of resident CTAs (three an SM) times a segment's
-// length smallest.  A segment's summary costs a quarter of its walk.  8 x 1024 tokens of 5120 channels: 1.08 ms, in one piece 1.54;
+// length smallest; pieces of fewer than 64 tokens only while all are in one wave (1024 tokens of 300 channels: 44 us, 60 with pieces of 64;
+// 8 x 128 of 4096 in one piece 128, in three 148).  A segment's summary costs a quarter of its walk.  8 x 1024 tokens of 5120 channels: 1.08 ms, in one piece 1.54;
 // 16384 of 2048 fp32: 0.93 ms in 27 segments, 1.05 in 24, 1.13 with eight states a lane.  Where even the most segments leave an SM fewer
-// than six warps, eight a lane (4 x 256 tokens of 1536 channels: 79 us against 89; 16 x 64 of 2048, seven warps: 77 against 69).
+// than eight warps, eight a lane (2 x 333 tokens of 1536 channels: 66 us against 72; 4 x 256, ten warps: 79 against 73).
 // Up to 64 states lie on eight lanes of two channels (2 x 1024 tokens of 5120 channels: 1.13 ms; sixteen a lane of one channel, with twice
 // the reads of B and C: 1.76).
 Plan plan_bwd(int batch, int seqlen, int dim, int groups, int dstate) {
   const int64_t sms = sm_count();
   Plan p = dstate <= 16 ? share_of(batch, dim, groups, 8, 2, 2) : dstate <= 32 ? share_of(batch, dim, groups, 8, 2, 4) : share_of(batch, dim, groups, 8, 2, 8);
-  if (dstate <= 32 && (int64_t)batch * p.tiles * std::min(kMaxSegs, std::max(1, seqlen / kMinSeg)) < 6 * sms) p = share_of(batch, dim, groups, 8, 1, p.q);
+  if (dstate <= 32 && (int64_t)batch * p.tiles * std::min(kMaxSegs, std::max(1, seqlen / kMinSeg)) < 8 * sms) p = share_of(batch, dim, groups, 8, 1, p.q);
   const int64_t ctas = std::max<int64_t>(1, (int64_t)batch * groups * ceil_div(p.tpg, kBwdWarps)), slots = (p.ch == 2 ? 3 : 4) * sms;
   int64_t best = 1;
   double least = 0.0;
   for (int64_t n = 1; n <= std::min<int64_t>(kMaxSegs, std::max(1, seqlen / kMinSeg)); ++n) {
+    if (seqlen / n < 2 * kMinSeg && n > 1 && ctas * n > slots) break;
     const double cost = (double)ceil_div(ctas * n, slots) / n * (1.0 + 0.25 * (n - 1) / n);
     if (n == 1 || cost < least) { least = cost; best = n; }
   }
