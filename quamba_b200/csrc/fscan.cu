@@ -286,7 +286,7 @@ template <typename G, typename P>
 __device__ __forceinline__ void load_record(const P* rec, int lane, f2 (&h)[G::kCh][G::kPairs]) {
 #pragma unroll
   for (int i = 0; i < G::kCh * G::kPairs; i += 2) {
-    const ulonglong2 v = *(reinterpret_cast<const ulonglong2*>(rec) + (i / 2) * 32 + lane);
+    const ulonglong2 v = __ldcg(reinterpret_cast<const ulonglong2*>(rec) + (i / 2) * 32 + lane);   // see grid_dependency_wait()
     h[i / G::kPairs][i % G::kPairs] = v.x;
     h[i / G::kPairs][i % G::kPairs + 1] = v.y;
   }
@@ -331,7 +331,7 @@ __device__ __forceinline__ void fold(const float* sum, const Place<G>& w, const 
   load_record<G>(sum, w.lane, loc);
 #pragma unroll
   for (int c = 0; c < G::kCh; ++c) {
-    const float d = sum[G::kRec + w.cg * G::kCh + c];
+    const float d = __ldcg(sum + G::kRec + w.cg * G::kCh + c);
 #pragma unroll
     for (int p = 0; p < G::kPairs; ++p) h[c][p] = fma2(exp2_pair(mul2(pack2(d, d), A[c][p])), h[c][p], loc[c][p]);
   }
@@ -467,10 +467,6 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
   f2 A[G::kCh][G::kPairs], h[G::kCh][G::kPairs];
   load_A(a, w, A);
   load_state(kOut ? a.initial_state : nullptr, a, w, h);
-  if (kOut)
-#pragma unroll 4
-    for (int i = 0; i < w.seg; ++i) fold(sums + (((int64_t)w.b * nseg + i) * tiles + w.tile) * G::kSum, w, A, h);
-
   const T* const xp = static_cast<const T*>(kRev ? a.dy : a.x) + (int64_t)w.b * (kRev ? a.dy_sb : a.x_sb) + w.ch0;
   const T* const dp = static_cast<const T*>(a.dt) + (int64_t)w.b * a.dt_sb + w.ch0;
   const T* const zp = a.z != nullptr && kMode != 1 ? static_cast<const T*>(a.z) + (int64_t)w.b * a.z_sb + w.ch0 : nullptr;
@@ -490,10 +486,17 @@ float_scan_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int nse
   const bool has_D = a.D != nullptr;
   T* const yp = kOut ? static_cast<T*>(a.y) + (int64_t)w.b * a.seqlen * a.dim + w.ch0 + c4 : nullptr;
 
+  // The summaries' kernel lets the one that reads them in as it starts: everything up to the first tile's copy overlaps its end.
+  if (!kOut) grid_dependency_launch();
   const int count = (int)((end - begin + kT - 1) / kT);
   auto tile_start = [&](int i) { return begin + (kRev ? count - 1 - i : i) * kT; };
   if (count > 0) stage_tile<T, G, kT, 3>(s.raw[0], src, stride, bc, bc_stride, tile_start(0), end, w.nch, a.dstate, vec, lane);
   copy_commit();
+  if (kOut && nseg > 1) {
+    grid_dependency_wait();
+#pragma unroll 4
+    for (int i = 0; i < w.seg; ++i) fold(sums + (((int64_t)w.b * nseg + i) * tiles + w.tile) * G::kSum, w, A, h);
+  }
   for (int i = 0; i < count; ++i) {
     const int t0 = tile_start(i);
     auto& raw = s.raw[i & 1];
@@ -722,6 +725,8 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
   f2 A[G::kCh][G::kPairs], carry[G::kCh][G::kPairs], dA[G::kCh][G::kPairs];
   load_A(a, w, A);
   load_state(a.d_final, a, w, carry);
+  grid_dependency_launch();
+  if (nseg > 1) grid_dependency_wait();
 #pragma unroll 4
   for (int i = nseg - 1; i > w.seg; --i) fold(sums + (((int64_t)w.b * nseg + i) * tiles + w.tile) * G::kSum, w, A, carry);
 #pragma unroll
@@ -982,13 +987,15 @@ float_scan_bwd_kernel(const __grid_constant__ qb_float_scan_args a, int tpg, int
 // dB and dC: the CTAs' sums added up in their order
 template <typename T>
 __global__ void __launch_bounds__(256) float_scan_bc_kernel(const __grid_constant__ qb_float_scan_args a, const float* part, int cpg, int npad) {
+  grid_dependency_launch();
+  grid_dependency_wait();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;      // (b, t, group, B | C, n)
   const int n = (int)(i % npad), k = (int)(i / npad % 2), g = (int)(i / (2 * npad) % a.groups);
   const int64_t bt = i / ((int64_t)2 * npad * a.groups), tokens = (int64_t)a.batch * a.seqlen;
   if (bt >= tokens || n >= a.dstate) return;
   const float* p = part + ((int64_t)g * cpg * tokens + bt) * (2 * npad) + k * npad + n;
   float v = 0.0f;
-  for (int c = 0; c < cpg; ++c) v += p[(int64_t)c * tokens * (2 * npad)];
+  for (int c = 0; c < cpg; ++c) v += __ldcg(p + (int64_t)c * tokens * (2 * npad));
   T* out = static_cast<T*>(k ? a.d_C : a.d_B);
   if (out != nullptr) out[(bt * a.groups + g) * a.dstate + n] = from_f<T>(v);
 }
@@ -997,6 +1004,7 @@ __global__ void __launch_bounds__(256) float_scan_bc_kernel(const __grid_constan
 template <typename G>
 __global__ void __launch_bounds__(G::kGrad) float_scan_param_kernel(const __grid_constant__ qb_float_scan_args a, const float* part, int tpg, int runs) {
   constexpr int kRec = G::kRec, kGrad = G::kGrad, kNp = G::kNp;
+  grid_dependency_wait();
   const int tiles = tpg * a.groups, tile = (int)blockIdx.x, i = (int)threadIdx.x;
   const int per = a.dim / a.groups, c0 = (tile % tpg) * G::kWc, ch0 = tile / tpg * per + c0, nch = min(G::kWc, per - c0);
   const bool is_A = i < kRec;
@@ -1006,7 +1014,7 @@ __global__ void __launch_bounds__(G::kGrad) float_scan_param_kernel(const __grid
   if (ch >= nch || (is_A && n >= a.dstate)) return;
   const float* p = part + (int64_t)tile * kGrad + i;
   float sum = 0.0f;
-  for (int r = 0; r < runs; ++r) sum += p[(int64_t)r * tiles * kGrad];
+  for (int r = 0; r < runs; ++r) sum += __ldcg(p + (int64_t)r * tiles * kGrad);
   if (is_A) {
     if (a.d_A != nullptr) a.d_A[(int64_t)(ch0 + ch) * a.dstate + n] = sum;
   } else if (i < kRec + 32) {
@@ -1225,7 +1233,8 @@ int launch_scan(const qb_float_scan_args& a, const Plan& p, float* sums, Vec vec
   });
   if (rc != QB_OK) return rc;
   const int64_t grid = (int64_t)a.batch * (p.nseg - (kMode == 0 ? 0 : 1)) * p.tiles;
-  float_scan_kernel<T, G, kMode><<<(unsigned)grid, 32, smem, st>>>(a, p.tpg, p.nseg, p.seg_len, sums, vec);
+  if (kMode == 0 && p.nseg > 1) launch_dependent(float_scan_kernel<T, G, kMode>, dim3((unsigned)grid), dim3(32), smem, st, a, p.tpg, p.nseg, p.seg_len, sums, vec);
+  else float_scan_kernel<T, G, kMode><<<(unsigned)grid, 32, smem, st>>>(a, p.tpg, p.nseg, p.seg_len, sums, vec);
   QB_LAUNCH_OK("float_scan_kernel");
   return QB_OK;
 }
@@ -1262,16 +1271,17 @@ int run_bwd(const qb_float_scan_args& a, const Plan& p, cudaStream_t st) {
   const int cpg = (int)ceil_div(p.tpg, kBwdWarps);
   if (a.batch > 0) {
     const int64_t grid = (int64_t)a.batch * p.nseg * cpg * a.groups;
-    float_scan_bwd_kernel<T, G><<<(unsigned)grid, 32 * kBwdWarps, smem, st>>>(a, p.tpg, p.nseg, p.seg_len, sums, part, grad, vec);
+    if (p.nseg > 1) launch_dependent(float_scan_bwd_kernel<T, G>, dim3((unsigned)grid), dim3(32 * kBwdWarps), smem, st, a, p.tpg, p.nseg, p.seg_len, sums, part, grad, vec);
+    else float_scan_bwd_kernel<T, G><<<(unsigned)grid, 32 * kBwdWarps, smem, st>>>(a, p.tpg, p.nseg, p.seg_len, sums, part, grad, vec);
     QB_LAUNCH_OK("float_scan_bwd_kernel");
   }
   const int64_t cells = (int64_t)a.batch * a.seqlen * a.groups * 2 * G::kN;
   if (cells > 0 && (a.d_B != nullptr || a.d_C != nullptr)) {
-    float_scan_bc_kernel<T><<<(unsigned)ceil_div(cells, 256), 256, 0, st>>>(a, part, cpg, G::kN);
+    launch_dependent(float_scan_bc_kernel<T>, dim3((unsigned)ceil_div(cells, 256)), dim3(256), 0, st, a, part, cpg, G::kN);
     QB_LAUNCH_OK("float_scan_bc_kernel");
   }
   if (a.d_A != nullptr || a.d_D != nullptr || a.d_bias != nullptr) {
-    float_scan_param_kernel<G><<<(unsigned)p.tiles, G::kGrad, 0, st>>>(a, grad, p.tpg, a.batch * p.nseg);
+    launch_dependent(float_scan_param_kernel<G>, dim3((unsigned)p.tiles), dim3(G::kGrad), 0, st, a, grad, p.tpg, a.batch * p.nseg);
     QB_LAUNCH_OK("float_scan_param_kernel");
   }
   return QB_OK;
