@@ -11,6 +11,7 @@
 // (token, channel) and SM, while its bytes (8 at 16 bits) take 0.18 clocks of HBM time.
 #include <algorithm>
 #include <cstddef>
+#include <type_traits>
 #include "tc_common.cuh"
 
 namespace qb {
@@ -1025,68 +1026,79 @@ __global__ void __launch_bounds__(G::kGrad) float_scan_param_kernel(const __grid
 }
 
 // ---- one token --------------------------------------------------------------------------------------------------------------
-// Bound by the state, read and written once (8 bytes per state).  kLanes lanes of a channel hold four states each and walk `rows`
-// sequences, kAhead at a time: all loads first, so that enough is under way.  What a (sequence, channel) costs besides its
+// Bound by the state, read and written once (8 bytes per state): 256 sequences of 5120 channels of 16 states 37 us (4.5 TB/s), 64 12 us;
+// what is left are the latencies of a turn (eight warps more an SM or the next turn's states in L2 already change nothing).  kLanes lanes
+// of a channel hold four states each and walk `rows` sequences, kAhead at a time: all loads first, none of them widened or asked for under
+// a condition, which would wait for each in turn (52 us).  Two at a time and eight CTAs an SM: four and six 39 us.  What a (sequence, channel) costs besides its
 // states -- loads, softplus, gate, output -- a lane does for its own share of the kAhead sequences only, and passes delta and delta x round.
-constexpr int kAhead = 4;
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(128, 6) float_update_kernel(const __grid_constant__ qb_float_update_args a, int rows, int vec, int vec_bc) {
+constexpr int kAhead = 2, kUpdateBlocks = 8;
+// Four values as whole registers, where they lie together.
+template <typename T> struct Packed { using type = uint2; };
+template <> struct Packed<float> { using type = float4; };
+template <bool kVec, typename T>
+__device__ __forceinline__ typename Packed<T>::type load_packed(const T* p, int count) {
+  using R = typename Packed<T>::type;
+  if constexpr (kVec) {
+    return *reinterpret_cast<const R*>(p);
+  } else {
+    __align__(16) T v[4] = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < count) v[k] = p[k];
+    return *reinterpret_cast<const R*>(v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void widen(const typename Packed<T>::type& r, f2& lo, f2& hi) {
+  __align__(16) T v[4];
+  *reinterpret_cast<typename Packed<T>::type*>(v) = r;
+  lo = pack2(to_f(v[0]), to_f(v[1]));
+  hi = pack2(to_f(v[2]), to_f(v[3]));
+}
+template <typename T, int kLanes, bool kVec>
+__global__ void __launch_bounds__(128, kUpdateBlocks) float_update_kernel(const __grid_constant__ qb_float_update_args a, int rows) {
   constexpr int kOwners = kLanes < kAhead ? kLanes : kAhead, kOwn = kAhead / kOwners;
   const int i = (int)blockIdx.x * 128 + (int)threadIdx.x;
-  const int sub = i % kLanes, n0 = sub * 4, d = min(i / kLanes, a.dim - 1), g = d / (a.dim / a.groups);   // the last lanes repeat the last channel
+  const int sub = i % kLanes, n0 = min(sub * 4, kVec ? a.dstate - 4 : 64), count = a.dstate - sub * 4, d = min(i / kLanes, a.dim - 1), g = d / (a.dim / a.groups);   // the last lanes repeat the last channel
   const bool mine = i / kLanes == d;
   f2 A[2];
   {
     float v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = n0 + k < a.dstate ? a.A[(int64_t)d * a.dstate + n0 + k] * kLog2e : 0.0f;
+    for (int k = 0; k < 4; ++k) v[k] = k < count ? a.A[(int64_t)d * a.dstate + n0 + k] * kLog2e : 0.0f;
     A[0] = pack2(v[0], v[1]);
     A[1] = pack2(v[2], v[3]);
   }
   const float bias = a.dt_bias != nullptr ? a.dt_bias[d] : 0.0f, Dv = a.D != nullptr ? a.D[d] : 0.0f;
   const int b0 = (int)blockIdx.y * rows, b1 = min(a.batch, b0 + rows), own0 = min(sub, kOwners - 1) * kOwn;
-  const float* st = a.state + b0 * a.state_sb + (int64_t)d * a.state_sd + n0;
-  float* so = a.state_out + b0 * a.state_out_sb + (int64_t)d * a.state_out_sd + n0;
-  const T* Bp = static_cast<const T*>(a.Bm) + b0 * a.B_sb + (int64_t)g * a.B_sg + n0;
-  const T* Cp = static_cast<const T*>(a.Cm) + b0 * a.C_sb + (int64_t)g * a.C_sg + n0;
+  const float* st = a.state + (int64_t)d * a.state_sd + n0;
+  float* so = a.state_out + (int64_t)d * a.state_out_sd + n0;
+  const T* Bp = static_cast<const T*>(a.Bm) + (int64_t)g * a.B_sg + n0;
+  const T* Cp = static_cast<const T*>(a.Cm) + (int64_t)g * a.C_sg + n0;
   for (int c0 = b0; c0 < b1; c0 += kAhead) {
-    float4 h[kAhead], B[kAhead], C[kAhead];
+    float4 h[kAhead];
+    typename Packed<T>::type B[kAhead], C[kAhead];
+    T xr[kOwn], dr[kOwn], zr[kOwn];
     float x[kOwn], dl[kOwn], z[kOwn], u[kOwn], own_y[kOwn];
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
       const int64_t b = min(c0 + own0 + k, b1 - 1);      // past the last: the last again
-      x[k] = to_f(static_cast<const T*>(a.x)[b * a.x_sb + d]);
-      dl[k] = to_f(static_cast<const T*>(a.dt)[b * a.dt_sb + d]);
-      z[k] = a.z != nullptr ? to_f(static_cast<const T*>(a.z)[b * a.z_sb + d]) : 0.0f;
+      xr[k] = static_cast<const T*>(a.x)[b * a.x_sb + d];
+      dr[k] = static_cast<const T*>(a.dt)[b * a.dt_sb + d];
+      zr[k] = a.z != nullptr ? static_cast<const T*>(a.z)[b * a.z_sb + d] : from_f<T>(0.0f);
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      h[k] = B[k] = C[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (c0 + k < b1) {
-        if (vec) {
-          if (n0 < a.dstate) h[k] = *reinterpret_cast<const float4*>(st);
-        } else {
-          if (n0 < a.dstate) h[k].x = st[0];
-          if (n0 + 1 < a.dstate) h[k].y = st[1];
-          if (n0 + 2 < a.dstate) h[k].z = st[2];
-          if (n0 + 3 < a.dstate) h[k].w = st[3];
-        }
-        if (vec_bc) {
-          if (n0 < a.dstate) { B[k] = quad(Bp); C[k] = quad(Cp); }
-        } else {
-          if (n0 < a.dstate) { B[k].x = to_f(Bp[0]); C[k].x = to_f(Cp[0]); }
-          if (n0 + 1 < a.dstate) { B[k].y = to_f(Bp[1]); C[k].y = to_f(Cp[1]); }
-          if (n0 + 2 < a.dstate) { B[k].z = to_f(Bp[2]); C[k].z = to_f(Cp[2]); }
-          if (n0 + 3 < a.dstate) { B[k].w = to_f(Bp[3]); C[k].w = to_f(Cp[3]); }
-        }
-      }
-      st += a.state_sb;
-      Bp += a.B_sb;
-      Cp += a.C_sb;
+      const int64_t b = min(c0 + k, b1 - 1);
+      h[k] = load_packed<kVec>(st + b * a.state_sb, count);
+      B[k] = load_packed<kVec>(Bp + b * a.B_sb, count);
+      C[k] = load_packed<kVec>(Cp + b * a.C_sb, count);
     }
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
-      dl[k] += bias;
+      x[k] = to_f(xr[k]);
+      z[k] = to_f(zr[k]);
+      dl[k] = to_f(dr[k]) + bias;
       float twin = dl[k];
       if (a.dt_softplus) softplus_series(dl[k], twin);
       u[k] = dl[k] * x[k];
@@ -1095,11 +1107,14 @@ __global__ void __launch_bounds__(128, 6) float_update_kernel(const __grid_const
     for (int k = 0; k < kAhead; ++k) {
       // one decay a call: what is systematic in it would add up over calls (see make_up())
       const f2 dd = splat(__shfl_sync(0xffffffffu, dl[k % kOwn], k / kOwn, kLanes)), uu = splat(__shfl_sync(0xffffffffu, u[k % kOwn], k / kOwn, kLanes));
-      const f2 h0 = fma2(exp2_fine(mul2(dd, A[0])), pack2(h[k].x, h[k].y), mul2(uu, pack2(B[k].x, B[k].y)));
-      const f2 h1 = fma2(exp2_fine(mul2(dd, A[1])), pack2(h[k].z, h[k].w), mul2(uu, pack2(B[k].z, B[k].w)));
+      f2 in0, in1, out0, out1;
+      widen<T>(B[k], in0, in1);
+      widen<T>(C[k], out0, out1);
+      const f2 h0 = fma2(exp2_fine(mul2(dd, A[0])), pack2(h[k].x, h[k].y), mul2(uu, in0));
+      const f2 h1 = fma2(exp2_fine(mul2(dd, A[1])), pack2(h[k].z, h[k].w), mul2(uu, in1));
       float y, y1;
-      unpack2(fma2(h1, pack2(C[k].z, C[k].w), mul2(h0, pack2(C[k].x, C[k].y))), y, y1);
-      y += y1;
+      unpack2(fma2(h1, out1, mul2(h0, out0)), y, y1);
+      y = count > 0 ? y + y1 : 0.0f;
 #pragma unroll
       for (int o = 1; o < kLanes; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
       if (k / kOwn == min(sub, kOwners - 1)) own_y[k % kOwn] = y;
@@ -1107,16 +1122,16 @@ __global__ void __launch_bounds__(128, 6) float_update_kernel(const __grid_const
         float4 r;
         unpack2(h0, r.x, r.y);
         unpack2(h1, r.z, r.w);
-        if (vec) {
-          if (n0 < a.dstate) *reinterpret_cast<float4*>(so) = r;
+        float* to = so + (c0 + k) * a.state_out_sb;
+        if (kVec) {
+          if (count > 0) *reinterpret_cast<float4*>(to) = r;
         } else {
-          if (n0 < a.dstate) so[0] = r.x;
-          if (n0 + 1 < a.dstate) so[1] = r.y;
-          if (n0 + 2 < a.dstate) so[2] = r.z;
-          if (n0 + 3 < a.dstate) so[3] = r.w;
+          if (0 < count) to[0] = r.x;
+          if (1 < count) to[1] = r.y;
+          if (2 < count) to[2] = r.z;
+          if (3 < count) to[3] = r.w;
         }
       }
-      so += a.state_out_sb;
     }
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
@@ -1359,25 +1374,30 @@ extern "C" int qb_float_scan_update(const qb_float_update_args* a, void* stream)
   if (a->batch == 0) return QB_OK;
   const int lanes = a->dstate <= 4 ? 1 : a->dstate <= 8 ? 2 : a->dstate <= 16 ? 4 : a->dstate <= 32 ? 8 : 16;
   const int64_t across = ceil_div((int64_t)a->dim * lanes, 128);
-  // sequences of a thread: as many as leave every SM six CTAs, in whole turns of kAhead (64 x 5120 x 16 states: 17 us, one each 37)
-  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(a->batch, ceil_div(across * a->batch, 6 * sm_count())));
+  // sequences of a thread, in whole turns of kAhead: as many as make all CTAs resident at once
+  const int64_t share = ceil_div(a->batch, std::min<int64_t>(a->batch, std::max<int64_t>(1, kUpdateBlocks * sm_count() / across)));
   const int64_t rows = share > 2 ? ceil_div(share, kAhead) * kAhead : share, down = ceil_div(a->batch, rows);
   QB_REQUIRE(across < (1ll << 24) && down < 65536, QB_ERR_TOO_LARGE, "float_scan_update: batch and dim are too large");
   const size_t size = a->dtype == 0 ? 4 : 2;
-  const int vec = a->dstate % 4 == 0 && aligned(a->state, 16) && aligned(a->state_out, 16) &&
-                  (a->state_sb | a->state_sd | a->state_out_sb | a->state_out_sd) % 4 == 0;
-  const int vec_bc = a->dstate % 4 == 0 && aligned(a->Bm, 4 * size) && aligned(a->Cm, 4 * size) && (a->B_sb | a->B_sg | a->C_sb | a->C_sg) % 4 == 0;
+  const bool vec = a->dstate % 4 == 0 && aligned(a->state, 16) && aligned(a->state_out, 16) &&
+                   (a->state_sb | a->state_sd | a->state_out_sb | a->state_out_sd) % 4 == 0 &&
+                   aligned(a->Bm, 4 * size) && aligned(a->Cm, 4 * size) && (a->B_sb | a->B_sg | a->C_sb | a->C_sg) % 4 == 0;
   return by_type(a->dtype, [&](auto t) -> int {
     using T = decltype(t);
     cudaStream_t st = (cudaStream_t)stream;
     const dim3 g((unsigned)across, (unsigned)down);
-    switch (lanes) {
-      case 1: float_update_kernel<T, 1><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc); break;
-      case 2: float_update_kernel<T, 2><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc); break;
-      case 4: float_update_kernel<T, 4><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc); break;
-      case 8: float_update_kernel<T, 8><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc); break;
-      default: float_update_kernel<T, 16><<<g, 128, 0, st>>>(*a, (int)rows, vec, vec_bc);
-    }
+    const auto go = [&](auto lanes_, auto vec_) {
+      float_update_kernel<T, decltype(lanes_)::value, decltype(vec_)::value><<<g, 128, 0, st>>>(*a, (int)rows);
+    };
+    const auto pick = [&](auto vec_) {
+      if (lanes == 1) go(std::integral_constant<int, 1>{}, vec_);
+      else if (lanes == 2) go(std::integral_constant<int, 2>{}, vec_);
+      else if (lanes == 4) go(std::integral_constant<int, 4>{}, vec_);
+      else if (lanes == 8) go(std::integral_constant<int, 8>{}, vec_);
+      else go(std::integral_constant<int, 16>{}, vec_);
+    };
+    if (vec) pick(std::true_type{});
+    else pick(std::false_type{});
     QB_LAUNCH_OK("float_update_kernel");
     return QB_OK;
   });
