@@ -1029,8 +1029,8 @@ __global__ void __launch_bounds__(G::kGrad) float_scan_param_kernel(const __grid
 // Bound by the state, read and written once (8 bytes per state): 256 sequences of 5120 channels of 16 states 37 us (4.5 TB/s), 64 12 us;
 // what is left are the latencies of a turn (eight warps more an SM or the next turn's states in L2 already change nothing).  kLanes lanes
 // of a channel hold four states each and walk `rows` sequences, kAhead at a time: all loads first, none of them widened or asked for under
-// a condition, which would wait for each in turn (52 us).  Two at a time and eight CTAs an SM: four and six 39 us.  What a (sequence, channel) costs besides its
-// states -- loads, softplus, gate, output -- a lane does for its own share of the kAhead sequences only, and passes delta and delta x round.
+// a condition, which would wait for each in turn (52 us).  Two at a time and eight CTAs an SM: four and six 39 us.  What a (sequence,
+// channel) costs besides its states -- loads, softplus, gate, output -- a lane does for its own share of the kAhead sequences only, and passes delta and delta x round.
 constexpr int kAhead = 2, kUpdateBlocks = 8;
 // Four values as whole registers, where they lie together.
 template <typename T> struct Packed { using type = uint2; };
@@ -1167,9 +1167,9 @@ void cut(Plan& p, int seqlen, int64_t want) {
   p.nseg = (int)std::max<int64_t>(1, ceil_div(seqlen, p.seg_len));
 }
 // Forward.  Eight states a lane: sixteen take fewer instructions but leave too few warps on an SM to hide each one's latencies
-// (8 x 1024 tokens of 5120 channels: 374 us against 440).  More than 32 states: eight of two channels, as on the way back (2 x 1024 tokens of
+// (8 x 1024 tokens of 5120 channels: 367 us against 440).  More than 32 states: eight of two channels, as on the way back (2 x 1024 tokens of
 // 5120 channels: 409 us, sixteen of one channel 511, eight of one 689).  Rows that put fewer than eight warps on an SM are cut into segments, which are
-// walked twice (512 tokens of 1536 channels: 25 us, in one piece 68; 4 x 2048 of 5120, nine warps: 488, cut in four 532).  Pieces of 32
+// walked twice (512 tokens of 1536 channels: 23 us, in one piece 68; 4 x 2048 of 5120, nine warps: 482, cut in four 532).  Pieces of 32
 // tokens are the shortest (2 x 333 tokens of 1536 channels: 28 us, of 64 34, of 16 27, but 4 x 256 33, 38 and 36).  What fewer than six warps
 // an SM are left of then takes four states a lane.
 Plan plan_fwd(int batch, int seqlen, int dim, int groups, int dstate) {
@@ -1183,8 +1183,8 @@ Plan plan_fwd(int batch, int seqlen, int dim, int groups, int dstate) {
 }
 // Backward: sixteen states a lane, in as many segments as make the number of waves of resident CTAs (three an SM) times a segment's
 // length smallest; pieces of fewer than 64 tokens only while all are in one wave (1024 tokens of 300 channels: 44 us, 60 with pieces of 64;
-// 8 x 128 of 4096 in one piece 128, in three 148).  A segment's summary costs a quarter of its walk.  8 x 1024 tokens of 5120 channels: 1.08 ms, in one piece 1.54;
-// 16384 of 2048 fp32: 0.93 ms in 27 segments, 1.05 in 24, 1.13 with eight states a lane.  Where even the most segments leave an SM fewer
+// 8 x 128 of 4096 in one piece 128, in three 148).  A segment's summary costs a quarter of its walk.  8 x 1024 tokens of 5120 channels:
+// 1.07 ms, in one piece 1.54; 16384 of 2048 fp32: 0.93 ms in 27 segments, 1.05 in 24, 1.13 with eight states a lane.  Where even the most segments leave an SM fewer
 // than eight warps, eight a lane (2 x 333 tokens of 1536 channels: 66 us against 72; 4 x 256, ten warps: 79 against 73).
 // Up to 64 states lie on eight lanes of two channels (2 x 1024 tokens of 5120 channels: 1.13 ms; sixteen a lane of one channel, with twice
 // the reads of B and C: 1.76).
@@ -1356,7 +1356,7 @@ extern "C" int qb_float_scan_bwd(const qb_float_scan_args* a, void* stream) {
   QB_REQUIRE((a->dy != nullptr && a->checkpoints != nullptr) || (int64_t)a->batch * a->seqlen == 0, QB_ERR_INVALID_ARG, "float_scan_bwd: dy and checkpoints are needed");
   QB_REQUIRE(aligned(a->checkpoints, 16), QB_ERR_INVALID_ARG, "float_scan_bwd: checkpoints must be 16-byte aligned");
   const Plan p = plan_of(a->batch, a->seqlen, a->dim, a->groups, a->dstate, true);
-  const int64_t need = qb_float_scan_workspace_bytes(a->batch, a->seqlen, a->dim, a->groups, a->dstate, 1);
+  const int64_t need = sums_bytes(p, a->batch) + part_bytes(p, a->batch, a->seqlen, a->groups) + grad_bytes(p, a->batch);
   QB_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need && aligned(a->workspace, 16)), QB_ERR_INVALID_ARG,
              "float_scan_bwd: the workspace must have %lld bytes, 16-byte aligned", (long long)need);
   return by_type(a->dtype, [&](auto t) -> int {
